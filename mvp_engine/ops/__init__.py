@@ -26,6 +26,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _ext
+from .muon import muon_lr_ratio, muon_step_, orthogonalize
 
 __all__ = [
     "gemm",
@@ -45,6 +46,9 @@ __all__ = [
     "bias_gelu",
     "vision_rope_pad",
     "bias_residual",
+    "orthogonalize",
+    "muon_step_",
+    "muon_lr_ratio",
 ]
 
 

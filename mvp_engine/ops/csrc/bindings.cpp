@@ -103,6 +103,14 @@ torch::Tensor bias_grad(const torch::Tensor& g, const c10::optional<torch::Tenso
 torch::Tensor vision_rope_bwd(const torch::Tensor& dq, const torch::Tensor& dk, const torch::Tensor& dv,
                               const torch::Tensor& cosv, const torch::Tensor& sinv, int64_t D);
 
+void orthogonalize(const torch::Tensor& x, torch::Tensor& out, int64_t steps, const std::vector<double>& coefficients,
+                   double eps, int64_t status_ptr);
+void muon_step_(const std::vector<torch::Tensor>& p, const std::vector<torch::Tensor>& g,
+                const std::vector<torch::Tensor>& mom, const std::vector<torch::Tensor>& p_bf16, double rate,
+                double decay, double momentum, bool nesterov, int64_t steps, const std::vector<double>& coefficients,
+                double eps, double grad_scale, const c10::optional<torch::Tensor>& norm_sq, double max_norm,
+                int64_t status_ptr);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "mvp_engine sm_100a kernels";
   m.def("gemm", &gemm_sm100, "tcgen05 bf16 GEMM C (+)= A * B^T with K- or MN-major operands");
@@ -155,4 +163,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("peer_publish", &peer_publish, "publish a sequence number into every rank's signal slot");
   m.def("peer_slot_sum_f32", &peer_slot_sum_f32,
         "publish, wait for every rank, then sum fp32 partial slots [W, n] into bf16 [n]");
+  m.def("orthogonalize", &orthogonalize, "Newton-Schulz orthogonalisation of a stack of matrices");
+  m.def("muon_step_", &muon_step_, "momentum, orthogonalised update and weights of same-shaped matrices", py::arg("p"),
+        py::arg("g"), py::arg("mom"), py::arg("p_bf16"), py::arg("rate"), py::arg("decay"), py::arg("momentum"),
+        py::arg("nesterov"), py::arg("steps"), py::arg("coefficients"), py::arg("eps"), py::arg("grad_scale"),
+        py::arg("norm_sq"), py::arg("max_norm"), py::arg("status_ptr"));
 }

@@ -1,0 +1,906 @@
+// Orthogonalisation of update matrices by Newton-Schulz products, and the optimizer step built on it.
+//
+//   X <- u / max(|u|_F, eps)
+//   repeat `steps` times, over the short side s = min(m, n):
+//     A = X X^T (m <= n) or X^T X (m > n)          [s, s], symmetric
+//     B = b A + c A A                              [s, s], symmetric
+//     X <- a X + B X (or a X + X B)                [m, n]
+//   O = X;   step: p <- p (1 - lr wd) - lr adj O
+//
+// Numbers.  The products run on the tensor core in fp16 with fp32 accumulation.  Rounding X to 16 bits would
+// put white noise of relative size r into every singular direction, and the linear term multiplies what lies in
+// the weak ones by a = 3.44 per iteration, 485 times in five: for a matrix with a fast decaying spectrum bf16
+// (r = 2^-9 on average) ends 10 to 20 % off and fp16 1 to 3 %.  So the linear term a X is exact to 22 bits: X is kept as
+// the sum of two fp16 values (hi + lo), the epilogue adds a (hi + lo) to the fp32 accumulator, and only hi goes
+// into the products, whose part of the result is small while a weak direction is.  All spectra tried then end
+// within 1.5e-3 of 64-bit arithmetic before the final rounding.
+// fp16's range is met by fixed powers of two: |X|_F <= 1 at the start makes the mean square of X sigma = 2^k,
+// k = round(log2(m n) / 2), equal to about 1, and A, B (trace <= 1 at first) are stored times tau = 2^round(log2 s).
+// A and B are close to multiples of the identity once X is nearly orthogonal, so their diagonals are kept in fp32 and
+// only what is off them is rounded to fp16: with A = D + A~, A A = A~ A~ + (D_i + D_j) A~ + D^2 element by element, and
+// B's diagonal joins the linear term, (a + B_ii) (hi + lo).  That halves the error of well conditioned matrices
+// (simulated against 64 bits at 512 x 2048: 1.7e-3 -> 0.5e-3) and bounds it for tiny ones.
+// Entries then stay below 1.9 sigma and 3.9 tau (the caller checks the coefficients for it), within 65504, and
+// what underflows is 2^-24 of an average entry.
+//
+// Work.  A and A A are symmetric: only tiles on and below the diagonal are computed, and the epilogue writes a
+// tile and its mirror, which makes an iteration s^2 l + s^3 + 2 s^2 l operations instead of 4 s^2 l + 2 s^3.
+// One launch per product handles a whole stack of same-shaped matrices.  The kernel is the pair-of-SMs GEMM
+// (256 x 256 tile per cluster, see gemm2sm_sm100.cu for the roles) over 3-D tensor maps.
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include <cmath>
+
+#include "common.cuh"
+#include "pair_sm100.cuh"
+#include "tma_host.h"
+
+namespace mvp {
+namespace muon {
+
+using namespace gemm2;
+
+constexpr int BK = 64;
+constexpr int TILE = 256;
+constexpr int HALF = 128;
+constexpr int STAGES = 6;
+constexpr int OP_BYTES = HALF * BK * 2;  // 16 KB of A and 16 KB of B per stage and CTA
+constexpr int STAGE_BYTES = 2 * OP_BYTES;
+constexpr int TMEM_COLS = 512;
+constexpr int THREADS = 192;
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
+constexpr int kMaxStack = 64;  // matrices per launch (their pointers travel as kernel parameters)
+
+// What the epilogue does with the fp32 accumulator `acc` of a tile.
+enum Epi : int {
+  kGram = 0,   // A: D = alpha acc, tile and mirror of a symmetric product; its diagonal goes to diag, in fp32
+  kPoly = 1,   // B: D = alpha acc + (beta + gamma (a_m + a_n)) C with A's diagonal a; as above
+  kNext = 2,   // X: D_hi + D_lo = alpha acc + (beta + diag) (C_hi + C_lo)
+  kOut = 3,    // out[b] = alpha acc + (beta + diag) (C_hi + C_lo), in the output's type
+  kStep = 4,   // p[b] = decay p[b] - rate (alpha acc + (beta + diag) (C_hi + C_lo)), and its bf16 copy
+};
+
+struct Outs {
+  void* out[kMaxStack];               // kOut: the results; kStep: fp32 master weights
+  __nv_bfloat16* shadow[kMaxStack];   // kStep: bf16 copies, or null
+};
+
+struct Params {
+  int M, N, K, count;   // per matrix: D [M, N], reduction K; matrices in the stack
+  int tiles;            // tiles per matrix
+  float alpha, beta;
+  const __half* C_hi;   // element-wise term, row stride ld, matrix stride ld * M
+  const __half* C_lo;
+  __half* D_hi;
+  __half* D_lo;
+  int ld;               // of C and D (a multiple of 8, at least N)
+  float* diag;          // [count, ld_s] diagonal of D (kGram, kPoly: written, and zeroed in D) or of B (others: added
+  int ld_s;             // to beta, times diag_scale, for row m where X is short by rows, else for column n)
+  float diag_scale;
+  const float* diag_a;  // kPoly: A's diagonal
+  float gamma, tau;
+  float decay, rate;
+  int* status;
+};
+
+__device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const void* tmap, uint32_t bar, int c0, int c1,
+                                                 int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
+// Instruction descriptor of kind::f16 with fp16 operands (A and B format 0) and fp32 accumulate.
+__host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N, bool a_mn_major, bool b_mn_major) {
+  return (1u << 4) | ((a_mn_major ? 1u : 0u) << 15) | ((b_mn_major ? 1u : 0u) << 16) |
+         ((static_cast<uint32_t>(N) >> 3) << 17) | ((static_cast<uint32_t>(M) >> 4) << 24);
+}
+
+// Tile t of a matrix: the lower triangle row by row for symmetric products, else 8-row groups.
+template <bool SYM>
+__device__ __forceinline__ void tile_of(const Params& p, int t, int& tm, int& tn) {
+  if constexpr (SYM) {
+    tm = static_cast<int>((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
+    while (tm * (tm + 1) / 2 > t) --tm;
+    while ((tm + 1) * (tm + 2) / 2 <= t) ++tm;
+    tn = t - tm * (tm + 1) / 2;
+  } else {
+    const int num_m = (p.M + TILE - 1) / TILE, num_n = (p.N + TILE - 1) / TILE;
+    constexpr int kGroup = 8;
+    const int per_group = kGroup * num_n;
+    const int g = t / per_group, first = g * kGroup;
+    const int gm = min(kGroup, num_m - first);
+    const int r = t - g * per_group;
+    tm = first + r % gm;
+    tn = r / gm;
+  }
+}
+
+__device__ __forceinline__ float2 h2f(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+__device__ __forceinline__ uint32_t f2h(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+template <bool A_MN, bool B_MN, int EPI, typename OUT>
+__global__ void __launch_bounds__(THREADS, 1)
+    ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p,
+                      const __grid_constant__ Outs outs) {
+  constexpr bool SYM = EPI == kGram || EPI == kPoly;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + STAGES * OP_BYTES;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);  // used in the leader
+  uint64_t* empty_bar = full_bar + STAGES;                                        // both CTAs
+  uint64_t* tfull_bar = empty_bar + STAGES;                                       // [2] both CTAs
+  uint64_t* tempty_bar = tfull_bar + 2;                                           // [2] used in the leader
+  uint64_t* done_bar = tempty_bar + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  const uint32_t crank = cluster_ctarank();  // 0 = leader
+  const int cluster_id = blockIdx.x >> 1;
+  const int clusters = gridDim.x >> 1;
+  const int num_kb = (p.K + BK - 1) / BK;
+  const int total = p.tiles * p.count;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull_bar[a], 1);
+      mbar_init(&tempty_bar[a], 2 * 128);  // epilogue threads of both CTAs
+    }
+    mbar_init(done_bar, 1);
+    *abort_flag = 0;
+    fence_mbarrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync_all();  // barriers of both CTAs initialised before any remote arrive / copy
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer (both CTAs)
+    if (elect_one_sync()) {
+      const uint32_t leader_full0 = mapa_shared(smem_u32(&full_bar[0]), 0);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true, issued = false;
+      for (int t = cluster_id; ok && t < total; t += clusters) {
+        const int b = t / p.tiles;
+        int tm, tn;
+        tile_of<SYM>(p, t - b * p.tiles, tm, tn);
+        const int m0 = tm * TILE + crank * HALF, n0 = tn * TILE + crank * HALF;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1, abort_flag, p.status, kTimeoutProducer)) {
+            ok = false;
+            break;
+          }
+          if (crank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * STAGE_BYTES);
+          issued = true;
+          const uint32_t bar = leader_full0 + stage * 8;
+          uint8_t* a_dst = sA + stage * OP_BYTES;
+          uint8_t* b_dst = sB + stage * OP_BYTES;
+          const int k0 = kb * BK;
+          if constexpr (!A_MN) {
+            tma_load_3d_pair(a_dst, &tmA, bar, k0, m0, b);
+          } else {
+            tma_load_3d_pair(a_dst, &tmA, bar, m0, k0, b);
+            tma_load_3d_pair(a_dst + 64 * BK * 2, &tmA, bar, m0 + 64, k0, b);
+          }
+          if constexpr (!B_MN) {
+            tma_load_3d_pair(b_dst, &tmB, bar, k0, n0, b);
+          } else {
+            tma_load_3d_pair(b_dst, &tmB, bar, n0, k0, b);
+            tma_load_3d_pair(b_dst + 64 * BK * 2, &tmB, bar, n0 + 64, k0, b);
+          }
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      // After an abort, let copies already issued into this CTA's ring land (bounded) before exit.
+      if ((!ok || *abort_flag) && issued) {
+        const uint64_t t0 = globaltimer();
+        while (globaltimer() - t0 < 200000000ull) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ----------------------------------------------------------------- MMA (leader only)
+    if (crank == 0 && elect_one_sync()) {
+      constexpr uint32_t idesc = make_idesc_f16(TILE, TILE, A_MN, B_MN);
+      int stage = 0;
+      uint32_t phase = 0;
+      int local = 0;
+      bool ok = true;
+      for (int t = cluster_id; ok && t < total; t += clusters, ++local) {
+        const int acc = local & 1;
+        const uint32_t acc_phase = (local >> 1) & 1;
+        if (!mbar_wait_bounded(&tempty_bar[acc], acc_phase ^ 1, abort_flag, p.status, kTimeoutMma)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * TILE;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait_bounded(&full_bar[stage], phase, abort_flag, p.status, kTimeoutMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a_base = smem_u32(sA + stage * OP_BYTES);
+          const uint32_t b_base = smem_u32(sB + stage * OP_BYTES);
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k) {
+            uint64_t adesc, bdesc;
+            if constexpr (!A_MN) adesc = make_smem_desc_sw128(a_base + k * 32, 16, 1024);
+            else adesc = make_smem_desc_sw128(a_base + k * 2048, 64 * BK * 2, 1024);
+            if constexpr (!B_MN) bdesc = make_smem_desc_sw128(b_base + k * 32, 16, 1024);
+            else bdesc = make_smem_desc_sw128(b_base + k * 2048, 64 * BK * 2, 1024);
+            mma_pair(d_tmem, adesc, bdesc, idesc, (kb != 0 || k != 0) ? 1u : 0u);
+          }
+          mma_commit_pair(&empty_bar[stage]);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        mma_commit_pair(&tfull_bar[acc]);
+      }
+      mma_commit_pair_local(done_bar);
+      mbar_wait_bounded(done_bar, 0, abort_flag, p.status, kTimeoutDrain);
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue (both CTAs)
+    const int sub = warp & 3;
+    const int row_in_tile = crank * HALF + sub * 32 + lane;
+    const uint32_t leader_tempty0 = mapa_shared(smem_u32(&tempty_bar[0]), 0);
+    int local = 0;
+    for (int t = cluster_id; t < total; t += clusters, ++local) {
+      const int b = t / p.tiles;
+      int tm, tn;
+      tile_of<SYM>(p, t - b * p.tiles, tm, tn);
+      const int acc = local & 1;
+      const uint32_t acc_phase = (local >> 1) & 1;
+      if (!__all_sync(0xffffffffu,
+                      mbar_wait_bounded(&tfull_bar[acc], acc_phase, abort_flag, p.status, kTimeoutEpilogue)))
+        break;
+      tc_fence_after();
+      const int m = tm * TILE + row_in_tile;
+      const bool row_ok = m < p.M;
+      const int64_t mat = static_cast<int64_t>(b) * p.M * p.ld;
+      const int64_t row = mat + static_cast<int64_t>(m) * p.ld;
+      constexpr bool kDiagByColumn = !SYM && !B_MN;  // X B: the diagonal belongs to X's columns
+      float beta = p.beta;
+      if constexpr (!SYM && !kDiagByColumn)
+        if (row_ok) beta += p.diag_scale * p.diag[static_cast<int64_t>(b) * p.ld_s + m];
+      float a_row = 0.f;
+      if constexpr (EPI == kPoly) {
+        if (row_ok) a_row = p.diag_a[static_cast<int64_t>(b) * p.ld_s + m];
+        beta += p.gamma * a_row;
+      }
+#pragma unroll 1
+      for (int c = 0; c < TILE / 32; ++c) {
+        const int n = tn * TILE + c * 32;
+        if (n >= p.N) break;  // the rest of the tile is outside the matrix (same for all lanes)
+        // the element-wise term: columns up to ld may be read and written, those beyond N are never used
+        uint4 hi[4], lo[4];
+        const bool has_c = row_ok && EPI != kGram;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          hi[v] = lo[v] = make_uint4(0u, 0u, 0u, 0u);
+          if (has_c && n + 8 * v < p.ld) {
+            hi[v] = *reinterpret_cast<const uint4*>(p.C_hi + row + n + 8 * v);
+            if constexpr (!SYM) lo[v] = *reinterpret_cast<const uint4*>(p.C_lo + row + n + 8 * v);
+          }
+        }
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(sub * 32) << 16) + acc * TILE + c * 32, r);
+        tmem_wait_ld();
+        float x[32];
+        float beta_col = 0.f;  // lane j: what column n + j adds to beta
+        if constexpr (EPI == kPoly)
+          beta_col = n + lane < p.N ? p.gamma * p.diag_a[static_cast<int64_t>(b) * p.ld_s + n + lane] : 0.f;
+        if constexpr (kDiagByColumn)
+          beta_col = n + lane < p.N ? p.diag_scale * p.diag[static_cast<int64_t>(b) * p.ld_s + n + lane] : 0.f;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const uint32_t* h = &hi[v].x;
+          const uint32_t* l = &lo[v].x;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float2 e = h2f(h[q]);
+            if constexpr (!SYM) {
+              const float2 f = h2f(l[q]);
+              e.x += f.x;
+              e.y += f.y;
+            }
+            const int j = 8 * v + 2 * q;
+            constexpr bool kByColumn = kDiagByColumn || EPI == kPoly;
+            const float b0 = kByColumn ? beta + __shfl_sync(0xffffffffu, beta_col, j) : beta;
+            const float b1 = kByColumn ? beta + __shfl_sync(0xffffffffu, beta_col, j + 1) : beta;
+            if constexpr (EPI == kGram) e = make_float2(0.f, 0.f);
+            x[j] = fmaf(b0, e.x, p.alpha * __uint_as_float(r[j]));
+            x[j + 1] = fmaf(b1, e.y, p.alpha * __uint_as_float(r[j + 1]));
+          }
+        }
+        if constexpr (SYM) {
+          if (row_ok && tm == tn) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (n + j == m) {
+                // tau times the diagonal element: A's comes out of the sum, B's adds b a + c a^2 (C is zero there)
+                if constexpr (EPI == kPoly) x[j] = fmaf(p.tau * a_row, p.beta + p.gamma * a_row, x[j]);
+                p.diag[static_cast<int64_t>(b) * p.ld_s + m] = x[j] / p.tau;
+                x[j] = 0.f;
+              }
+          }
+          uint32_t h[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) h[j] = f2h(x[2 * j], x[2 * j + 1]);
+          if (row_ok) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+              if (n + 8 * v < p.ld)
+                *reinterpret_cast<uint4*>(p.D_hi + row + n + 8 * v) =
+                    make_uint4(h[4 * v], h[4 * v + 1], h[4 * v + 2], h[4 * v + 3]);
+            if (tm != tn) {  // mirror: a warp's 32 rows are 64 contiguous bytes of each mirrored row
+              __half* d = p.D_hi + mat + static_cast<int64_t>(n) * p.ld + m;
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (n + j < p.N) {
+                  const __half2 pair = *reinterpret_cast<const __half2*>(&h[j / 2]);
+                  d[static_cast<int64_t>(j) * p.ld] = (j & 1) ? __high2half(pair) : __low2half(pair);
+                }
+            }
+          }
+        } else if constexpr (EPI == kNext) {
+          if (row_ok) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              uint32_t h[4], l[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const float u0 = x[8 * v + 2 * q], u1 = x[8 * v + 2 * q + 1];
+                h[q] = f2h(u0, u1);
+                const float2 back = h2f(h[q]);
+                l[q] = f2h(u0 - back.x, u1 - back.y);
+              }
+              if (n + 8 * v < p.ld) {
+                *reinterpret_cast<uint4*>(p.D_hi + row + n + 8 * v) = make_uint4(h[0], h[1], h[2], h[3]);
+                *reinterpret_cast<uint4*>(p.D_lo + row + n + 8 * v) = make_uint4(l[0], l[1], l[2], l[3]);
+              }
+            }
+          }
+        } else if constexpr (EPI == kOut) {
+          if (row_ok) {
+            OUT* d = static_cast<OUT*>(outs.out[b]) + static_cast<int64_t>(m) * p.N + n;
+            if (n + 32 <= p.N && (reinterpret_cast<uintptr_t>(d) & 15) == 0) {
+              if constexpr (sizeof(OUT) == 4) {
+#pragma unroll
+                for (int v = 0; v < 8; ++v)
+                  reinterpret_cast<float4*>(d)[v] = make_float4(x[4 * v], x[4 * v + 1], x[4 * v + 2], x[4 * v + 3]);
+              } else {
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                  __align__(16) OUT e[8];
+#pragma unroll
+                  for (int q = 0; q < 8; ++q) e[q] = from_f32<OUT>(x[8 * v + q]);
+                  reinterpret_cast<uint4*>(d)[v] = *reinterpret_cast<const uint4*>(e);
+                }
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (n + j < p.N) d[j] = from_f32<OUT>(x[j]);
+            }
+          }
+        } else {
+          if (row_ok) {
+            const int64_t off = static_cast<int64_t>(m) * p.N + n;
+            float* w = static_cast<float*>(outs.out[b]) + off;
+            __nv_bfloat16* s = outs.shadow[b] != nullptr ? outs.shadow[b] + off : nullptr;
+            const bool full = n + 32 <= p.N;
+            if (full && (reinterpret_cast<uintptr_t>(w) & 15) == 0) {
+#pragma unroll
+              for (int v = 0; v < 8; ++v) {
+                float4 o = reinterpret_cast<const float4*>(w)[v];
+                o.x = x[4 * v] = fmaf(-p.rate, x[4 * v], p.decay * o.x);
+                o.y = x[4 * v + 1] = fmaf(-p.rate, x[4 * v + 1], p.decay * o.y);
+                o.z = x[4 * v + 2] = fmaf(-p.rate, x[4 * v + 2], p.decay * o.z);
+                o.w = x[4 * v + 3] = fmaf(-p.rate, x[4 * v + 3], p.decay * o.w);
+                reinterpret_cast<float4*>(w)[v] = o;
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (n + j < p.N) w[j] = x[j] = fmaf(-p.rate, x[j], p.decay * w[j]);
+            }
+            if (s != nullptr) {
+              if (full && (reinterpret_cast<uintptr_t>(s) & 15) == 0) {
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                  reinterpret_cast<uint4*>(s)[v] =
+                      make_uint4(pack_bf16x2(x[8 * v], x[8 * v + 1]), pack_bf16x2(x[8 * v + 2], x[8 * v + 3]),
+                                 pack_bf16x2(x[8 * v + 4], x[8 * v + 5]), pack_bf16x2(x[8 * v + 6], x[8 * v + 7]));
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (n + j < p.N) s[j] = __float2bfloat16_rn(x[j]);
+              }
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      remote_arrive(leader_tempty0 + acc * 8);
+    }
+  }
+
+  // Both CTAs: every role is done (the leader's MMAs have retired); then free the pair's TMEM.
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------ norm and first X
+struct Ins {
+  const void* u[kMaxStack];  // the matrix (orthogonalize) or the gradient (step)
+  float* mom[kMaxStack];     // momentum buffers (step)
+};
+
+struct StartParams {
+  int rows, cols, ld;
+  int parts;           // partial sums per matrix
+  double* partial;     // [count, parts] sums of squares, added in index order by every reader
+  __half* hi;
+  __half* lo;
+  float sigma, eps;
+  float momentum;
+  int nesterov;
+  float grad_scale;
+  const float* norm_sq;
+  float max_norm;
+};
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// The gradient's factor: its scale times the global-norm clip coefficient (as in the AdamW kernel).
+__device__ __forceinline__ float grad_factor(const StartParams& p) {
+  float scale = p.grad_scale;
+  if (p.norm_sq != nullptr) {
+    const float total = sqrtf(*p.norm_sq) * p.grad_scale;
+    const float coef = p.max_norm / (total + 1e-6f);
+    scale *= (coef > 1.f) ? 1.f : coef;  // a NaN norm stays NaN
+  }
+  return scale;
+}
+
+// Block sum of doubles in a fixed order; the result is valid in thread 0.
+template <int THREADS_>
+__device__ __forceinline__ double block_sum(double s) {
+  __shared__ double red[THREADS_ / 32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    for (int w = 0; w < THREADS_ / 32; ++w) s += red[w];
+  }
+  return s;
+}
+
+constexpr int kStartThreads = 256;
+
+// Partial sums of squares of u (squares in 64 bits: the norm of values near the ends of fp32's range is right).
+// STEP: u is built here from the gradient and the momentum, which is updated.
+template <typename T, bool STEP>
+__global__ void __launch_bounds__(kStartThreads) ns_norm_kernel(const __grid_constant__ Ins ins, const StartParams p) {
+  const int b = blockIdx.y;
+  const int64_t n = static_cast<int64_t>(p.rows) * p.cols;
+  const T* g = static_cast<const T*>(ins.u[b]);
+  double s = 0.0;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kStartThreads;
+  if constexpr (STEP) {
+    float* mom = ins.mom[b];
+    const float scale = grad_factor(p);
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kStartThreads + threadIdx.x; i < n; i += stride) {
+      const float gi = to_f32(g[i]) * scale;
+      const float old = mom[i];
+      const float mi = old + (1.f - p.momentum) * (gi - old);
+      mom[i] = mi;
+      const float u = p.nesterov ? gi + p.momentum * (mi - gi) : mi;
+      s += static_cast<double>(u) * u;
+    }
+  } else {
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kStartThreads + threadIdx.x; i < n; i += stride) {
+      const double u = to_f32(g[i]);
+      s += u * u;
+    }
+  }
+  s = block_sum<kStartThreads>(s);
+  if (threadIdx.x == 0) p.partial[b * p.parts + blockIdx.x] = s;
+}
+
+// X = sigma u / max(|u|_F, eps) as hi + lo, rows padded with zeros to ld.
+template <typename T, bool STEP>
+__global__ void __launch_bounds__(kStartThreads) ns_first_kernel(const __grid_constant__ Ins ins, const StartParams p) {
+  __shared__ double factor_s;
+  const int b = blockIdx.y;
+  if (threadIdx.x < 32) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < p.parts; i += 32) s += p.partial[b * p.parts + i];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const double norm = sqrt(s);
+    // a norm that is not a number stays one
+    if (threadIdx.x == 0) factor_s = static_cast<double>(p.sigma) / (norm < p.eps ? static_cast<double>(p.eps) : norm);
+  }
+  __syncthreads();
+  const double factor = factor_s;
+  const T* g = static_cast<const T*>(ins.u[b]);
+  const float* mom = STEP ? ins.mom[b] : nullptr;
+  const float scale = STEP ? grad_factor(p) : 1.f;
+  const int groups = p.ld / 8;
+  const int64_t total = static_cast<int64_t>(p.rows) * groups;
+  const int64_t base = static_cast<int64_t>(b) * p.rows * p.ld;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kStartThreads + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * kStartThreads) {
+    const int64_t r = i / groups;
+    const int c = static_cast<int>(i - r * groups) * 8;
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = 0.f;
+      if (c + j < p.cols) {
+        const int64_t at = r * p.cols + c + j;
+        float u = to_f32(g[at]);
+        if constexpr (STEP) {
+          u *= scale;
+          const float mi = mom[at];
+          u = p.nesterov ? u + p.momentum * (mi - u) : mi;
+        }
+        x[j] = static_cast<float>(u * factor);
+      }
+    }
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      h[q] = f2h(x[2 * q], x[2 * q + 1]);
+      const float2 back = h2f(h[q]);
+      l[q] = f2h(x[2 * q] - back.x, x[2 * q + 1] - back.y);
+    }
+    *reinterpret_cast<uint4*>(p.hi + base + r * p.ld + c) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(p.lo + base + r * p.ld + c) = make_uint4(l[0], l[1], l[2], l[3]);
+  }
+}
+
+// ------------------------------------------------------------------------- host side
+// Tensor map of a stack [count, rows, cols] of fp16 matrices with row stride ld.
+inline void make_map(CUtensorMap* map, const __half* base, int cols, int rows, int count, int ld, bool mn_major) {
+  ensure_thread_context();
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(count)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * 2, static_cast<cuuint64_t>(ld) * 2 * rows};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(mn_major ? BK : HALF), 1};
+  cuuint32_t es[3] = {1, 1, 1};
+  const CUresult r = encode_tiled_fn()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(base), dims,
+                                       strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "orthogonalize: cuTensorMapEncodeTiled failed with code ", static_cast<int>(r));
+}
+
+template <bool A_MN, bool B_MN, int EPI, typename OUT = float>
+void product(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, const Outs& outs, int sms,
+             cudaStream_t stream) {
+  auto kern = ns_product_kernel<A_MN, B_MN, EPI, OUT>;
+  static std::atomic<uint64_t> configured{0};
+  allow_smem(kern, SMEM_BYTES, configured);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * std::min(p.tiles * p.count, std::max(1, sms / 2)));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, p, outs));
+}
+
+struct Shape {
+  int rows, cols, count;
+  int short_side, ldx, lds;
+  bool tall;
+  float sigma, tau;
+  Shape(int64_t m, int64_t n, int64_t L)
+      : rows(static_cast<int>(m)), cols(static_cast<int>(n)), count(static_cast<int>(L)) {
+    tall = m > n;
+    short_side = tall ? cols : rows;
+    ldx = (cols + 7) / 8 * 8;
+    lds = (short_side + 7) / 8 * 8;
+    sigma = std::ldexp(1.f, static_cast<int>(std::min(15.0, std::round(0.5 * std::log2(static_cast<double>(m) * n)))));
+    tau = std::ldexp(1.f, static_cast<int>(std::min(14.0, std::round(std::log2(static_cast<double>(short_side))))));
+  }
+  // fp16 elements of the workspace: X hi twice (a product reads one while its epilogue writes the other), X lo, A, B
+  int64_t x_elems() const { return static_cast<int64_t>(count) * rows * ldx; }
+  int64_t s_elems() const { return static_cast<int64_t>(count) * short_side * lds; }
+  int64_t elems() const { return 3 * x_elems() + 2 * s_elems(); }
+};
+
+struct Workspace {
+  torch::Tensor buf;
+  __half *hi[2], *lo, *A, *B;
+  float *diag_a, *diag_b;
+  Workspace(const Shape& s, const torch::Device& dev) {
+    const int64_t diag_elems = 4 * static_cast<int64_t>(s.count) * s.lds;  // two vectors of fp32
+    buf = torch::empty({s.elems() + diag_elems}, torch::TensorOptions().dtype(at::kHalf).device(dev));
+    hi[0] = reinterpret_cast<__half*>(buf.data_ptr());
+    hi[1] = hi[0] + s.x_elems();
+    lo = hi[1] + s.x_elems();
+    A = lo + s.x_elems();
+    B = A + s.s_elems();
+    diag_a = reinterpret_cast<float*>(B + s.s_elems());
+    diag_b = diag_a + static_cast<int64_t>(s.count) * s.lds;
+  }
+};
+
+// The iterations on a workspace whose hi[0] / lo hold the first X; `last` launches the final product.
+template <typename Last>
+void iterate(const Shape& s, Workspace& w, int steps, double a, double b, double c, int* status, int sms,
+             cudaStream_t stream, Last last) {
+  const int tiles_s = (s.short_side + TILE - 1) / TILE;
+  const int tiles_m = (s.rows + TILE - 1) / TILE, tiles_n = (s.cols + TILE - 1) / TILE;
+  const Outs none{};
+  CUtensorMap sa, sb;  // A and B as K-major operands (symmetric: rows are columns)
+  make_map(&sa, w.A, s.short_side, s.short_side, s.count, s.lds, false);
+  make_map(&sb, w.B, s.short_side, s.short_side, s.count, s.lds, false);
+  for (int it = 0; it < steps; ++it) {
+    const int cur = it & 1;
+    CUtensorMap xk, xmn;  // X as a K-major operand (rows) and as an MN-major one (columns)
+    make_map(&xk, w.hi[cur], s.cols, s.rows, s.count, s.ldx, false);
+    make_map(&xmn, w.hi[cur], s.cols, s.rows, s.count, s.ldx, true);
+    Params p{};
+    p.count = s.count;
+    p.status = status;
+    p.ld_s = s.lds;
+    p.tau = s.tau;
+    // A' = tau A = (tau / sigma^2) X' X'^T
+    p.M = p.N = s.short_side;
+    p.K = s.tall ? s.rows : s.cols;
+    p.tiles = tiles_s * (tiles_s + 1) / 2;
+    p.ld = s.lds;
+    p.alpha = s.tau / s.sigma / s.sigma;
+    p.beta = 0.f;
+    p.D_hi = w.A;
+    p.diag = w.diag_a;
+    if (s.tall) product<true, true, kGram>(xmn, xmn, p, none, sms, stream);
+    else product<false, false, kGram>(xk, xk, p, none, sms, stream);
+    // B' = tau (b A + c A A), off the diagonal (b + c (a_i + a_j)) A' + (c / tau) A' A' with A' zero on it
+    p.K = s.short_side;
+    p.alpha = static_cast<float>(c / s.tau);
+    p.beta = static_cast<float>(b);
+    p.C_hi = w.A;
+    p.D_hi = w.B;
+    p.gamma = static_cast<float>(c);
+    p.diag_a = w.diag_a;
+    p.diag = w.diag_b;
+    product<false, false, kPoly>(sa, sa, p, none, sms, stream);
+    // X' <- a X' + (1 / tau) B' X'   (or X' B')
+    p.M = s.rows;
+    p.N = s.cols;
+    p.K = s.short_side;
+    p.tiles = tiles_m * tiles_n;
+    p.ld = s.ldx;
+    p.alpha = 1.f / s.tau;
+    p.beta = static_cast<float>(a);
+    p.diag_scale = 1.f;
+    p.C_hi = w.hi[cur];
+    p.C_lo = w.lo;
+    if (it + 1 < steps) {
+      p.D_hi = w.hi[cur ^ 1];
+      p.D_lo = w.lo;  // in place: each element is read and written by one thread
+      if (s.tall) product<false, false, kNext>(xk, sb, p, none, sms, stream);
+      else product<false, true, kNext>(sb, xmn, p, none, sms, stream);
+    } else {
+      p.alpha /= s.sigma;
+      p.beta /= s.sigma;
+      p.diag_scale /= s.sigma;
+      last(s.tall ? xk : sb, s.tall ? sb : xmn, p);
+    }
+  }
+}
+
+// Matrices per group: bounded by the pointer table and by 2 GiB of workspace.
+inline int64_t group_size(int64_t rows, int64_t cols, int64_t count) {
+  const Shape one(rows, cols, 1);
+  const int64_t fit = std::max<int64_t>(1, (int64_t(1) << 30) / std::max<int64_t>(1, one.elems()));
+  return std::min<int64_t>(count, std::min<int64_t>(kMaxStack, fit));
+}
+
+inline StartParams start_params(const Shape& s, Workspace& w, torch::Tensor& partial, float eps) {
+  StartParams q{};
+  q.rows = s.rows;
+  q.cols = s.cols;
+  q.ld = s.ldx;
+  q.parts = static_cast<int>(partial.size(1));
+  q.partial = partial.data_ptr<double>();
+  q.hi = w.hi[0];
+  q.lo = w.lo;
+  q.sigma = s.sigma;
+  q.eps = eps;
+  q.grad_scale = 1.f;
+  return q;
+}
+
+// CTAs per matrix of the two start kernels: enough to fill the GPU eight times over the stack, at least 2048 values each.
+inline int start_ctas(const Shape& s, int sms) {
+  const int64_t n = static_cast<int64_t>(s.rows) * s.ldx;
+  const int64_t want = std::max<int64_t>(1, 8ll * sms / s.count);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, n / 2048)));
+}
+
+template <typename T, bool STEP>
+void start(const Ins& ins, const StartParams& q, const Shape& s, int ctas, cudaStream_t stream) {
+  ns_norm_kernel<T, STEP><<<dim3(q.parts, s.count), kStartThreads, 0, stream>>>(ins, q);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  ns_first_kernel<T, STEP><<<dim3(ctas, s.count), kStartThreads, 0, stream>>>(ins, q);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+void check_sizes(int64_t rows, int64_t cols, int64_t steps, const std::vector<double>& coefficients) {
+  TORCH_CHECK(rows > 0 && cols > 0 && rows < (1 << 30) && cols < (1 << 30), "orthogonalize: matrix sizes");
+  TORCH_CHECK(steps >= 1 && coefficients.size() == 3, "orthogonalize: at least one step, three coefficients");
+}
+
+template <typename OUT>
+void last_out(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, const Outs& o, bool tall, int sms,
+              cudaStream_t stream) {
+  if (tall) product<false, false, kOut, OUT>(ta, tb, p, o, sms, stream);
+  else product<false, true, kOut, OUT>(ta, tb, p, o, sms, stream);
+}
+
+}  // namespace muon
+}  // namespace mvp
+
+// O [count, m, n] of x [count, m, n] (contiguous fp32 / bf16 / fp16), in `out`'s type.
+void orthogonalize(const torch::Tensor& x, torch::Tensor& out, int64_t steps, const std::vector<double>& coefficients,
+                   double eps, int64_t status_ptr) {
+  using namespace mvp::muon;
+  TORCH_CHECK(x.is_cuda() && x.dim() == 3 && x.is_contiguous(), "orthogonalize: contiguous CUDA [count, m, n]");
+  TORCH_CHECK(out.is_cuda() && out.device() == x.device() && out.is_contiguous() && out.sizes() == x.sizes(),
+              "orthogonalize: contiguous output of the input's shape and device");
+  check_sizes(x.size(1), x.size(2), steps, coefficients);
+  const at::cuda::CUDAGuard guard(x.device());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  const int sms = mvp::num_sms(x.get_device());
+  const int64_t size = x.size(1) * x.size(2);
+  const int64_t group = group_size(x.size(1), x.size(2), x.size(0));
+  for (int64_t first = 0; first < x.size(0); first += group) {
+    const Shape s(x.size(1), x.size(2), std::min<int64_t>(group, x.size(0) - first));
+    Workspace w(s, x.device());
+    const int ctas = start_ctas(s, sms);
+    auto partial = torch::empty({s.count, ctas}, x.options().dtype(at::kDouble));
+    StartParams q = start_params(s, w, partial, static_cast<float>(eps));
+    Ins ins{};
+    Outs outs{};
+    for (int i = 0; i < s.count; ++i) {
+      ins.u[i] = static_cast<const char*>(x.data_ptr()) + (first + i) * size * x.element_size();
+      outs.out[i] = static_cast<char*>(out.data_ptr()) + (first + i) * size * out.element_size();
+    }
+    if (x.scalar_type() == at::kFloat) start<float, false>(ins, q, s, ctas, stream);
+    else if (x.scalar_type() == at::kBFloat16) start<__nv_bfloat16, false>(ins, q, s, ctas, stream);
+    else if (x.scalar_type() == at::kHalf) start<__half, false>(ins, q, s, ctas, stream);
+    else TORCH_CHECK(false, "orthogonalize: fp32, bf16 or fp16 input");
+    iterate(s, w, static_cast<int>(steps), coefficients[0], coefficients[1], coefficients[2],
+            reinterpret_cast<int*>(status_ptr), sms, stream,
+            [&](const CUtensorMap& ta, const CUtensorMap& tb, const Params& p) {
+              if (out.scalar_type() == at::kFloat) last_out<float>(ta, tb, p, outs, s.tall, sms, stream);
+              else if (out.scalar_type() == at::kBFloat16) last_out<__nv_bfloat16>(ta, tb, p, outs, s.tall, sms, stream);
+              else if (out.scalar_type() == at::kHalf) last_out<__half>(ta, tb, p, outs, s.tall, sms, stream);
+              else TORCH_CHECK(false, "orthogonalize: fp32, bf16 or fp16 output");
+            });
+  }
+}
+
+// One step on same-shaped fp32 matrices p (master), g (gradient), mom (momentum); see ops.muon_step_.
+void muon_step_(const std::vector<torch::Tensor>& p, const std::vector<torch::Tensor>& g,
+                const std::vector<torch::Tensor>& mom, const std::vector<torch::Tensor>& p_bf16, double rate,
+                double decay, double momentum, bool nesterov, int64_t steps, const std::vector<double>& coefficients,
+                double eps, double grad_scale, const c10::optional<torch::Tensor>& norm_sq, double max_norm,
+                int64_t status_ptr) {
+  using namespace mvp::muon;
+  if (p.empty()) return;
+  const size_t count = p.size();
+  TORCH_CHECK(g.size() == count && mom.size() == count && (p_bf16.empty() || p_bf16.size() == count),
+              "muon_step_: one gradient, momentum (and bf16 copy) per weight");
+  const auto dev = p[0].device();
+  const auto sizes = p[0].sizes();
+  TORCH_CHECK(p[0].is_cuda() && p[0].dim() == 2, "muon_step_: CUDA matrices");
+  auto check = [&](const torch::Tensor& t, at::ScalarType type, const char* what) {
+    TORCH_CHECK(t.device() == dev && t.scalar_type() == type && t.sizes() == sizes && t.is_contiguous(), "muon_step_: ",
+                what, " must be contiguous, of one shape, type and device");
+  };
+  for (size_t i = 0; i < count; ++i) {
+    check(p[i], at::kFloat, "fp32 weights");
+    check(g[i], at::kFloat, "fp32 gradients");
+    check(mom[i], at::kFloat, "fp32 momenta");
+    if (!p_bf16.empty()) check(p_bf16[i], at::kBFloat16, "bf16 copies");
+  }
+  TORCH_CHECK(!norm_sq.has_value() || (norm_sq->device() == dev && norm_sq->scalar_type() == at::kFloat &&
+                                       norm_sq->numel() == 1),
+              "muon_step_: norm_sq must be one fp32 value on the weights' device");
+  check_sizes(sizes[0], sizes[1], steps, coefficients);
+  const at::cuda::CUDAGuard guard(dev);
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  const int sms = mvp::num_sms(dev.index());
+  const int64_t group = group_size(sizes[0], sizes[1], static_cast<int64_t>(count));
+  for (int64_t first = 0; first < static_cast<int64_t>(count); first += group) {
+    const Shape s(sizes[0], sizes[1], std::min<int64_t>(group, static_cast<int64_t>(count) - first));
+    Workspace w(s, dev);
+    const int ctas = start_ctas(s, sms);
+    auto partial = torch::empty({s.count, ctas}, p[0].options().dtype(at::kDouble));
+    StartParams q = start_params(s, w, partial, static_cast<float>(eps));
+    q.momentum = static_cast<float>(momentum);
+    q.nesterov = nesterov ? 1 : 0;
+    q.grad_scale = static_cast<float>(grad_scale);
+    q.norm_sq = norm_sq.has_value() ? norm_sq->data_ptr<float>() : nullptr;
+    q.max_norm = static_cast<float>(max_norm);
+    Ins ins{};
+    Outs outs{};
+    for (int i = 0; i < s.count; ++i) {
+      ins.u[i] = g[first + i].data_ptr();
+      ins.mom[i] = mom[first + i].data_ptr<float>();
+      outs.out[i] = p[first + i].data_ptr();
+      outs.shadow[i] = p_bf16.empty() ? nullptr : reinterpret_cast<__nv_bfloat16*>(p_bf16[first + i].data_ptr());
+    }
+    start<float, true>(ins, q, s, ctas, stream);
+    iterate(s, w, static_cast<int>(steps), coefficients[0], coefficients[1], coefficients[2],
+            reinterpret_cast<int*>(status_ptr), sms, stream,
+            [&](const CUtensorMap& ta, const CUtensorMap& tb, Params l) {
+              l.rate = static_cast<float>(rate);
+              l.decay = static_cast<float>(decay);
+              if (s.tall) product<false, false, kStep>(ta, tb, l, outs, sms, stream);
+              else product<false, true, kStep>(ta, tb, l, outs, sms, stream);
+            });
+  }
+}

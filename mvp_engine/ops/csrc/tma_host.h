@@ -7,6 +7,7 @@
 #include <c10/util/Exception.h>
 
 #include <array>
+#include <atomic>
 #include <mutex>
 
 namespace mvp {
@@ -70,6 +71,18 @@ inline int num_sms(int device) {
     cache[device] = v > 0 ? v : 148;
   }
   return cache[device];
+}
+
+// Raises a kernel's dynamic shared-memory limit on the current device, once per device (`done`: one bit each).
+template <typename Kernel>
+inline void allow_smem(Kernel kern, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  TORCH_CHECK(e == cudaSuccess, "cudaFuncSetAttribute: ", cudaGetErrorString(e));
+  done.fetch_or(bit, std::memory_order_release);
 }
 
 }  // namespace mvp
