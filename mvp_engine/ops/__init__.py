@@ -26,6 +26,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _ext
+from .fp8 import Fp8Matrix, gemm_fp8, linear_fp8, quantize_fp8
 from .muon import muon_lr_ratio, muon_step_, orthogonalize
 
 __all__ = [
@@ -49,6 +50,10 @@ __all__ = [
     "orthogonalize",
     "muon_step_",
     "muon_lr_ratio",
+    "Fp8Matrix",
+    "quantize_fp8",
+    "gemm_fp8",
+    "linear_fp8",
 ]
 
 

@@ -26,6 +26,7 @@ KERNELS_PER_CALL = {
     "layernorm_fwd": 1, "layernorm_bwd": 3, "bias_gelu_fwd": 1, "bias_gelu_bwd": 2, "vision_rope_fwd": 1,
     "vision_rope_bwd": 1, "bias_residual_fwd": 1, "bias_grad": 2,
     "peer_gather_shards": 1, "publish_epoch": 1, "gemm_pair_gather": 1,
+    "quantize_fp8": 1, "gemm_fp8": 1,
     "orthogonalize": 17, "muon_step_": 17,  # norm, first X and three products for each of five iterations
 }
 launch_count = 0

@@ -111,6 +111,12 @@ void muon_step_(const std::vector<torch::Tensor>& p, const std::vector<torch::Te
                 double eps, double grad_scale, const c10::optional<torch::Tensor>& norm_sq, double max_norm,
                 int64_t status_ptr);
 
+void quantize_fp8(const torch::Tensor& x, bool tile, const c10::optional<torch::Tensor>& q,
+                  const c10::optional<torch::Tensor>& s, const c10::optional<torch::Tensor>& qt,
+                  const c10::optional<torch::Tensor>& st);
+void gemm_fp8(const torch::Tensor& a, const torch::Tensor& sa, const torch::Tensor& b, const torch::Tensor& sb,
+              torch::Tensor& c, bool accumulate, int64_t status_ptr);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "mvp_engine sm_100a kernels";
   m.def("gemm", &gemm_sm100, "tcgen05 bf16 GEMM C (+)= A * B^T with K- or MN-major operands");
@@ -168,4 +174,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("g"), py::arg("mom"), py::arg("p_bf16"), py::arg("rate"), py::arg("decay"), py::arg("momentum"),
         py::arg("nesterov"), py::arg("steps"), py::arg("coefficients"), py::arg("eps"), py::arg("grad_scale"),
         py::arg("norm_sq"), py::arg("max_norm"), py::arg("status_ptr"));
+  m.def("quantize_fp8", &quantize_fp8, "8-bit codes and block scales of a matrix's rows and / or columns");
+  m.def("gemm_fp8", &gemm_fp8, "C (+)= A * B^T of 8-bit matrices with a scale per block of 128 (tcgen05 block-scaled)");
 }
