@@ -256,6 +256,12 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
+// Programmatic dependent launch: a kernel launched with that attribute may start while the kernel before it in the
+// stream still runs; it may touch what that kernel writes (or reads) only after pdl_wait, which returns once the kernel
+// before it has completed and its writes are visible.  pdl_launch lets the next such kernel start.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ------------------------------------------------------- peer memory (NVLink)
 // Release / acquire at system scope: a flag another GPU reads (or writes) orders the data around it.
 __device__ __forceinline__ void st_release_sys(unsigned long long* p, unsigned long long v) {

@@ -48,12 +48,18 @@ using namespace gemm2;
 constexpr int BK = 64;
 constexpr int TILE = 256;
 constexpr int HALF = 128;
-constexpr int STAGES = 6;
+constexpr int STAGES = 5;
 constexpr int OP_BYTES = HALF * BK * 2;  // 16 KB of A and 16 KB of B per stage and CTA
 constexpr int STAGE_BYTES = 2 * OP_BYTES;
+constexpr int CHUNK = 32;                 // columns the epilogue handles at a time
+constexpr int CHUNKS = 128 / CHUNK;       // per warp and tile
+constexpr int HALF_BUF = 32 * CHUNK * 2;  // a warp's 32 rows of a chunk in fp16
+constexpr int EPI_BUF = 2 * HALF_BUF;     // hi and lo, or fp32
+constexpr int EPI_BYTES = 8 * 2 * EPI_BUF;  // two buffers for each warp
 constexpr int TMEM_COLS = 512;
-constexpr int THREADS = 192;
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
+constexpr int EPI_WARPS = 8;             // two for each quarter of the accumulator's lanes, half of the columns each
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + 1024 + 256;
 constexpr int kMaxStack = 64;  // matrices per launch (their pointers travel as kernel parameters)
 
 // What the epilogue does with the fp32 accumulator `acc` of a tile.
@@ -103,6 +109,13 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N, bool a_mn_ma
          ((static_cast<uint32_t>(N) >> 3) << 17) | ((static_cast<uint32_t>(M) >> 4) << 24);
 }
 
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void cp_async_wait_but_one() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
 // Tile t of a matrix: the lower triangle row by row for symmetric products, else 8-row groups.
 template <bool SYM>
 __device__ __forceinline__ void tile_of(const Params& p, int t, int& tm, int& tn) {
@@ -147,7 +160,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
   uint8_t* sB = smem + STAGES * OP_BYTES;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);  // used in the leader
+  uint8_t* sE = smem + STAGES * STAGE_BYTES;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sE + EPI_BYTES);               // used in the leader
   uint64_t* empty_bar = full_bar + STAGES;                                        // both CTAs
   uint64_t* tfull_bar = empty_bar + STAGES;                                       // [2] both CTAs
   uint64_t* tempty_bar = tfull_bar + 2;                                           // [2] used in the leader
@@ -170,7 +184,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull_bar[a], 1);
-      mbar_init(&tempty_bar[a], 2 * 128);  // epilogue threads of both CTAs
+      mbar_init(&tempty_bar[a], 2 * 32 * EPI_WARPS);  // epilogue threads of both CTAs
     }
     mbar_init(done_bar, 1);
     *abort_flag = 0;
@@ -188,6 +202,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   cluster_sync_all();  // barriers of both CTAs initialised before any remote arrive / copy
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  pdl_launch();
+  pdl_wait();  // every thread: what follows reads the product before this one, and writes what it may still read
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer (both CTAs)
@@ -282,110 +298,134 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs)
-    const int sub = warp & 3;
-    const int row_in_tile = crank * HALF + sub * 32 + lane;
+    // A warp takes its 32 rows in chunks of 32 columns.  tcgen05.ld gives a lane one row; global memory wants rows of
+    // consecutive lanes.  So both directions pass through a warp's own shared-memory buffer, in 16-byte pieces swizzled
+    // by row: the element-wise terms arrive by cp.async two chunks ahead (the first during the tile's MMAs), a lane
+    // combines its row, and 4 (fp16) or 8 (fp32) lanes write each row.
+    const int sub = warp & 3, ew = warp - 2;
+    uint8_t* const bufs = sE + ew * 2 * EPI_BUF;
     const uint32_t leader_tempty0 = mapa_shared(smem_u32(&tempty_bar[0]), 0);
+    const int row_in_tile = static_cast<int>(crank) * HALF + sub * 32;
+    const int col_in_tile = (ew / 4) * 128;
+    // byte offset of 16-byte piece j of row r: 64-byte rows (fp16) and 128-byte rows (fp32), both free of conflicts for
+    // lanes that read or write the same piece of 8 rows
+    auto piece16 = [](int r, int j) { return r * 64 + ((j ^ ((r >> 1) & 3)) << 4); };
+    auto piece32 = [](int r, int j) { return r * 128 + ((j ^ (r & 7)) << 4); };
+    auto fetch = [&](int seq) {  // element-wise terms of chunk `seq` of this warp's sequence
+      if constexpr (EPI != kGram) {
+        const int t = cluster_id + (seq / CHUNKS) * clusters;
+        if (t < total) {
+          const int b = t / p.tiles;
+          int tm, tn;
+          tile_of<SYM>(p, t - b * p.tiles, tm, tn);
+          const int n = tn * TILE + col_in_tile + (seq % CHUNKS) * CHUNK + (lane & 3) * 8;
+          const int64_t mat = static_cast<int64_t>(b) * p.M * p.ld;
+          const uint32_t dst = smem_u32(bufs + (seq & 1) * EPI_BUF);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + lane / 4, m = tm * TILE + row_in_tile + r;
+            const bool ok = m < p.M && n < p.ld;  // the columns between N and ld are never used
+            const int64_t at = ok ? mat + static_cast<int64_t>(m) * p.ld + n : 0;
+            const uint32_t d = dst + piece16(r, lane & 3);
+            cp_async_16(d, p.C_hi + at, ok ? 16 : 0);
+            if constexpr (!SYM) cp_async_16(d + HALF_BUF, p.C_lo + at, ok ? 16 : 0);
+          }
+        }
+        cp_async_commit();
+      }
+    };
+    fetch(0);
+    fetch(1);
     int local = 0;
     for (int t = cluster_id; t < total; t += clusters, ++local) {
       const int b = t / p.tiles;
       int tm, tn;
       tile_of<SYM>(p, t - b * p.tiles, tm, tn);
       const int acc = local & 1;
-      const uint32_t acc_phase = (local >> 1) & 1;
-      if (!__all_sync(0xffffffffu,
-                      mbar_wait_bounded(&tfull_bar[acc], acc_phase, abort_flag, p.status, kTimeoutEpilogue)))
-        break;
-      tc_fence_after();
-      const int m = tm * TILE + row_in_tile;
+      const int m_warp = tm * TILE + row_in_tile;  // the warp's first row
+      const int m = m_warp + lane;
       const bool row_ok = m < p.M;
       const int64_t mat = static_cast<int64_t>(b) * p.M * p.ld;
-      const int64_t row = mat + static_cast<int64_t>(m) * p.ld;
       constexpr bool kDiagByColumn = !SYM && !B_MN;  // X B: the diagonal belongs to X's columns
-      float beta = p.beta;
+      constexpr bool kByColumn = kDiagByColumn || EPI == kPoly;
+      const float* col_term = EPI == kPoly ? p.diag_a : p.diag;
+      const float col_scale = EPI == kPoly ? p.gamma : p.diag_scale;
+      float beta = p.beta, a_row = 0.f;
       if constexpr (!SYM && !kDiagByColumn)
         if (row_ok) beta += p.diag_scale * p.diag[static_cast<int64_t>(b) * p.ld_s + m];
-      float a_row = 0.f;
       if constexpr (EPI == kPoly) {
         if (row_ok) a_row = p.diag_a[static_cast<int64_t>(b) * p.ld_s + m];
         beta += p.gamma * a_row;
       }
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&tfull_bar[acc], (local >> 1) & 1, abort_flag, p.status,
+                                                     kTimeoutEpilogue)))
+        break;
+      tc_fence_after();
 #pragma unroll 1
-      for (int c = 0; c < TILE / 32; ++c) {
-        const int n = tn * TILE + c * 32;
-        if (n >= p.N) break;  // the rest of the tile is outside the matrix (same for all lanes)
-        // the element-wise term: columns up to ld may be read and written, those beyond N are never used
-        uint4 hi[4], lo[4];
-        const bool has_c = row_ok && EPI != kGram;
+      for (int c = 0; c < CHUNKS; ++c) {
+        const int seq = local * CHUNKS + c;
+        const int n = tn * TILE + col_in_tile + c * CHUNK;
+        uint8_t* const buf = bufs + (seq & 1) * EPI_BUF;
+        const bool live = n < p.N && m_warp < p.M;  // same for all lanes
+        float x[CHUNK];
+        if (live) {
+          uint32_t r[CHUNK];
+          tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(sub * 32) << 16) + acc * TILE + col_in_tile + c * CHUNK,
+                             r);
+          if constexpr (EPI != kGram) {
+            float by_col = 0.f;  // lane j: what column n + j adds to beta
+            if constexpr (kByColumn)
+              if (n + lane < p.N) by_col = col_scale * col_term[static_cast<int64_t>(b) * p.ld_s + n + lane];
+            cp_async_wait_but_one();
+            __syncwarp();
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          hi[v] = lo[v] = make_uint4(0u, 0u, 0u, 0u);
-          if (has_c && n + 8 * v < p.ld) {
-            hi[v] = *reinterpret_cast<const uint4*>(p.C_hi + row + n + 8 * v);
-            if constexpr (!SYM) lo[v] = *reinterpret_cast<const uint4*>(p.C_lo + row + n + 8 * v);
-          }
-        }
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(sub * 32) << 16) + acc * TILE + c * 32, r);
-        tmem_wait_ld();
-        float x[32];
-        float beta_col = 0.f;  // lane j: what column n + j adds to beta
-        if constexpr (EPI == kPoly)
-          beta_col = n + lane < p.N ? p.gamma * p.diag_a[static_cast<int64_t>(b) * p.ld_s + n + lane] : 0.f;
-        if constexpr (kDiagByColumn)
-          beta_col = n + lane < p.N ? p.diag_scale * p.diag[static_cast<int64_t>(b) * p.ld_s + n + lane] : 0.f;
+            for (int v = 0; v < 4; ++v) {
+              const uint8_t* at = buf + piece16(lane, v);
+              const uint4 hi = *reinterpret_cast<const uint4*>(at);
+              uint4 lo = make_uint4(0u, 0u, 0u, 0u);
+              if constexpr (!SYM) lo = *reinterpret_cast<const uint4*>(at + HALF_BUF);
+              const uint32_t* hw = &hi.x;
+              const uint32_t* lw = &lo.x;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const uint32_t* h = &hi[v].x;
-          const uint32_t* l = &lo[v].x;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float2 e = h2f(h[q]);
-            if constexpr (!SYM) {
-              const float2 f = h2f(l[q]);
-              e.x += f.x;
-              e.y += f.y;
-            }
-            const int j = 8 * v + 2 * q;
-            constexpr bool kByColumn = kDiagByColumn || EPI == kPoly;
-            const float b0 = kByColumn ? beta + __shfl_sync(0xffffffffu, beta_col, j) : beta;
-            const float b1 = kByColumn ? beta + __shfl_sync(0xffffffffu, beta_col, j + 1) : beta;
-            if constexpr (EPI == kGram) e = make_float2(0.f, 0.f);
-            x[j] = fmaf(b0, e.x, p.alpha * __uint_as_float(r[j]));
-            x[j + 1] = fmaf(b1, e.y, p.alpha * __uint_as_float(r[j + 1]));
-          }
-        }
-        if constexpr (SYM) {
-          if (row_ok && tm == tn) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (n + j == m) {
-                // tau times the diagonal element: A's comes out of the sum, B's adds b a + c a^2 (C is zero there)
-                if constexpr (EPI == kPoly) x[j] = fmaf(p.tau * a_row, p.beta + p.gamma * a_row, x[j]);
-                p.diag[static_cast<int64_t>(b) * p.ld_s + m] = x[j] / p.tau;
-                x[j] = 0.f;
-              }
-          }
-          uint32_t h[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) h[j] = f2h(x[2 * j], x[2 * j + 1]);
-          if (row_ok) {
-#pragma unroll
-            for (int v = 0; v < 4; ++v)
-              if (n + 8 * v < p.ld)
-                *reinterpret_cast<uint4*>(p.D_hi + row + n + 8 * v) =
-                    make_uint4(h[4 * v], h[4 * v + 1], h[4 * v + 2], h[4 * v + 3]);
-            if (tm != tn) {  // mirror: a warp's 32 rows are 64 contiguous bytes of each mirrored row
-              __half* d = p.D_hi + mat + static_cast<int64_t>(n) * p.ld + m;
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (n + j < p.N) {
-                  const __half2 pair = *reinterpret_cast<const __half2*>(&h[j / 2]);
-                  d[static_cast<int64_t>(j) * p.ld] = (j & 1) ? __high2half(pair) : __low2half(pair);
+              for (int q = 0; q < 4; ++q) {
+                float2 e = h2f(hw[q]);
+                if constexpr (!SYM) {
+                  const float2 f = h2f(lw[q]);
+                  e.x += f.x;
+                  e.y += f.y;
                 }
+                const int j = 8 * v + 2 * q;
+                x[j] = (kByColumn ? beta + __shfl_sync(0xffffffffu, by_col, j) : beta) * e.x;
+                x[j + 1] = (kByColumn ? beta + __shfl_sync(0xffffffffu, by_col, j + 1) : beta) * e.y;
+              }
+            }
+            __syncwarp();  // all rows of the buffer have been read
+          }
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < CHUNK; ++j)
+            x[j] = EPI == kGram ? p.alpha * __uint_as_float(r[j]) : fmaf(p.alpha, __uint_as_float(r[j]), x[j]);
+        }
+        if (c == CHUNKS - 1) {  // the accumulator has been read
+          tc_fence_before();
+          remote_arrive(leader_tempty0 + acc * 8);
+        }
+        if (live) {
+          if constexpr (SYM) {
+            if (n == m_warp) {  // the chunk on the diagonal: element j of lane j
+              float d = 0.f;
+#pragma unroll
+              for (int j = 0; j < CHUNK; ++j)
+                if (j == lane) {
+                  d = x[j];
+                  x[j] = 0.f;
+                }
+              // tau times the diagonal element: A's comes out of the sum, B's adds b a + c a^2 (C is zero there)
+              if constexpr (EPI == kPoly) d = fmaf(p.tau * a_row, p.beta + p.gamma * a_row, d);
+              if (row_ok) p.diag[static_cast<int64_t>(b) * p.ld_s + m] = d / p.tau;
             }
           }
-        } else if constexpr (EPI == kNext) {
-          if (row_ok) {
+          if constexpr (SYM || EPI == kNext) {
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
               uint32_t h[4], l[4];
@@ -396,75 +436,118 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const float2 back = h2f(h[q]);
                 l[q] = f2h(u0 - back.x, u1 - back.y);
               }
-              if (n + 8 * v < p.ld) {
-                *reinterpret_cast<uint4*>(p.D_hi + row + n + 8 * v) = make_uint4(h[0], h[1], h[2], h[3]);
-                *reinterpret_cast<uint4*>(p.D_lo + row + n + 8 * v) = make_uint4(l[0], l[1], l[2], l[3]);
+              uint8_t* at = buf + piece16(lane, v);
+              *reinterpret_cast<uint4*>(at) = make_uint4(h[0], h[1], h[2], h[3]);
+              if constexpr (!SYM) *reinterpret_cast<uint4*>(at + HALF_BUF) = make_uint4(l[0], l[1], l[2], l[3]);
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = i * 8 + lane / 4, col = n + (lane & 3) * 8;
+              const uint8_t* at = buf + piece16(r, lane & 3);
+              if (m_warp + r < p.M && col < p.ld) {
+                const int64_t d = mat + static_cast<int64_t>(m_warp + r) * p.ld + col;
+                *reinterpret_cast<uint4*>(p.D_hi + d) = *reinterpret_cast<const uint4*>(at);
+                if constexpr (!SYM) *reinterpret_cast<uint4*>(p.D_lo + d) = *reinterpret_cast<const uint4*>(at + HALF_BUF);
               }
             }
-          }
-        } else if constexpr (EPI == kOut) {
-          if (row_ok) {
-            OUT* d = static_cast<OUT*>(outs.out[b]) + static_cast<int64_t>(m) * p.N + n;
-            if (n + 32 <= p.N && (reinterpret_cast<uintptr_t>(d) & 15) == 0) {
-              if constexpr (sizeof(OUT) == 4) {
+            if constexpr (SYM) {
+              if (tm != tn && row_ok) {  // mirror: a warp's 32 rows are 64 contiguous bytes of each mirrored row
+                __half* d = p.D_hi + mat + static_cast<int64_t>(n) * p.ld + m;
 #pragma unroll
-                for (int v = 0; v < 8; ++v)
-                  reinterpret_cast<float4*>(d)[v] = make_float4(x[4 * v], x[4 * v + 1], x[4 * v + 2], x[4 * v + 3]);
-              } else {
+                for (int j = 0; j < CHUNK; ++j)
+                  if (n + j < p.N) d[static_cast<int64_t>(j) * p.ld] = __float2half_rn(x[j]);
+              }
+            }
+          } else if constexpr (EPI == kOut && sizeof(OUT) == 2) {
 #pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                  __align__(16) OUT e[8];
+            for (int v = 0; v < 4; ++v) {
+              __align__(16) OUT e[8];
 #pragma unroll
-                  for (int q = 0; q < 8; ++q) e[q] = from_f32<OUT>(x[8 * v + q]);
-                  reinterpret_cast<uint4*>(d)[v] = *reinterpret_cast<const uint4*>(e);
+              for (int q = 0; q < 8; ++q) e[q] = from_f32<OUT>(x[8 * v + q]);
+              *reinterpret_cast<uint4*>(buf + piece16(lane, v)) = *reinterpret_cast<const uint4*>(e);
+            }
+            __syncwarp();
+            OUT* out = static_cast<OUT*>(outs.out[b]);
+            if (p.N % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int r = i * 8 + lane / 4, col = n + (lane & 3) * 8;
+                if (m_warp + r < p.M && col < p.N)
+                  *reinterpret_cast<uint4*>(out + static_cast<int64_t>(m_warp + r) * p.N + col) =
+                      *reinterpret_cast<const uint4*>(buf + piece16(r, lane & 3));
+              }
+            } else {
+#pragma unroll 4
+              for (int r = 0; r < 32; ++r)
+                if (m_warp + r < p.M && n + lane < p.N)
+                  out[static_cast<int64_t>(m_warp + r) * p.N + n + lane] =
+                      *reinterpret_cast<const OUT*>(buf + piece16(r, lane / 8) + (lane & 7) * 2);
+            }
+          } else {
+#pragma unroll
+            for (int v = 0; v < 8; ++v)
+              *reinterpret_cast<float4*>(buf + piece32(lane, v)) =
+                  make_float4(x[4 * v], x[4 * v + 1], x[4 * v + 2], x[4 * v + 3]);
+            __syncwarp();
+            float* w = static_cast<float*>(outs.out[b]);
+            __nv_bfloat16* s = EPI == kStep ? outs.shadow[b] : nullptr;
+            if (p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0 && (reinterpret_cast<uintptr_t>(s) & 7) == 0) {
+              float4 o[8];
+              const int col = n + (lane & 7) * 4;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + lane / 8;
+                if (EPI == kStep && m_warp + r < p.M && col < p.N)
+                  o[i] = *reinterpret_cast<const float4*>(w + static_cast<int64_t>(m_warp + r) * p.N + col);
+              }
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + lane / 8;
+                if (m_warp + r >= p.M || col >= p.N) continue;
+                float4 u = *reinterpret_cast<const float4*>(buf + piece32(r, lane & 7));
+                const int64_t at = static_cast<int64_t>(m_warp + r) * p.N + col;
+                if constexpr (EPI == kStep) {
+                  u.x = fmaf(-p.rate, u.x, p.decay * o[i].x);
+                  u.y = fmaf(-p.rate, u.y, p.decay * o[i].y);
+                  u.z = fmaf(-p.rate, u.z, p.decay * o[i].z);
+                  u.w = fmaf(-p.rate, u.w, p.decay * o[i].w);
+                  if (s != nullptr)
+                    *reinterpret_cast<uint2*>(s + at) = make_uint2(pack_bf16x2(u.x, u.y), pack_bf16x2(u.z, u.w));
+                }
+                *reinterpret_cast<float4*>(w + at) = u;
+              }
+            } else {
+#pragma unroll 1
+              for (int r0 = 0; r0 < 32; r0 += 8) {
+                float o[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  if (EPI == kStep && m_warp + r0 + i < p.M && n + lane < p.N)
+                    o[i] = w[static_cast<int64_t>(m_warp + r0 + i) * p.N + n + lane];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const int r = r0 + i;
+                  if (m_warp + r >= p.M || n + lane >= p.N) continue;
+                  float u = *reinterpret_cast<const float*>(buf + piece32(r, lane / 4) + (lane & 3) * 4);
+                  const int64_t at = static_cast<int64_t>(m_warp + r) * p.N + n + lane;
+                  if constexpr (EPI == kStep) {
+                    u = fmaf(-p.rate, u, p.decay * o[i]);
+                    if (s != nullptr) s[at] = __float2bfloat16_rn(u);
+                  }
+                  w[at] = u;
                 }
               }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (n + j < p.N) d[j] = from_f32<OUT>(x[j]);
             }
           }
-        } else {
-          if (row_ok) {
-            const int64_t off = static_cast<int64_t>(m) * p.N + n;
-            float* w = static_cast<float*>(outs.out[b]) + off;
-            __nv_bfloat16* s = outs.shadow[b] != nullptr ? outs.shadow[b] + off : nullptr;
-            const bool full = n + 32 <= p.N;
-            if (full && (reinterpret_cast<uintptr_t>(w) & 15) == 0) {
-#pragma unroll
-              for (int v = 0; v < 8; ++v) {
-                float4 o = reinterpret_cast<const float4*>(w)[v];
-                o.x = x[4 * v] = fmaf(-p.rate, x[4 * v], p.decay * o.x);
-                o.y = x[4 * v + 1] = fmaf(-p.rate, x[4 * v + 1], p.decay * o.y);
-                o.z = x[4 * v + 2] = fmaf(-p.rate, x[4 * v + 2], p.decay * o.z);
-                o.w = x[4 * v + 3] = fmaf(-p.rate, x[4 * v + 3], p.decay * o.w);
-                reinterpret_cast<float4*>(w)[v] = o;
-              }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (n + j < p.N) w[j] = x[j] = fmaf(-p.rate, x[j], p.decay * w[j]);
-            }
-            if (s != nullptr) {
-              if (full && (reinterpret_cast<uintptr_t>(s) & 15) == 0) {
-#pragma unroll
-                for (int v = 0; v < 4; ++v)
-                  reinterpret_cast<uint4*>(s)[v] =
-                      make_uint4(pack_bf16x2(x[8 * v], x[8 * v + 1]), pack_bf16x2(x[8 * v + 2], x[8 * v + 3]),
-                                 pack_bf16x2(x[8 * v + 4], x[8 * v + 5]), pack_bf16x2(x[8 * v + 6], x[8 * v + 7]));
-              } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (n + j < p.N) s[j] = __float2bfloat16_rn(x[j]);
-              }
-            }
-          }
+        } else if constexpr (EPI != kGram) {
+          cp_async_wait_but_one();
         }
+        __syncwarp();  // the buffer has been written out
+        fetch(seq + 2);
       }
-      tc_fence_before();
-      remote_arrive(leader_tempty0 + acc * 8);
     }
+    if constexpr (EPI != kGram) cp_async_wait_all();
   }
 
   // Both CTAs: every role is done (the leader's MMAs have retired); then free the pair's TMEM.
@@ -529,31 +612,73 @@ __device__ __forceinline__ double block_sum(double s) {
 
 constexpr int kStartThreads = 256;
 
+__device__ __forceinline__ void load4(const float* p, float (&v)[4]) {
+  const float4 u = *reinterpret_cast<const float4*>(p);
+  v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+}
+template <typename H>
+__device__ __forceinline__ void load4(const H* p, float (&v)[4]) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  const H* h = reinterpret_cast<const H*>(&u);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = to_f32(h[j]);
+}
+// Whether a matrix (and its momentum) can be read four values at a time from its start.
+template <typename T, bool STEP>
+__device__ __forceinline__ bool aligned_for(const T* g, const float* mom) {
+  return reinterpret_cast<uintptr_t>(g) % (4 * sizeof(T)) == 0 && (!STEP || reinterpret_cast<uintptr_t>(mom) % 16 == 0);
+}
+
 // Partial sums of squares of u (squares in 64 bits: the norm of values near the ends of fp32's range is right).
 // STEP: u is built here from the gradient and the momentum, which is updated.
 template <typename T, bool STEP>
 __global__ void __launch_bounds__(kStartThreads) ns_norm_kernel(const __grid_constant__ Ins ins, const StartParams p) {
   const int b = blockIdx.y;
+  pdl_launch();  // launched without the attribute itself: the stream's earlier work is complete
   const int64_t n = static_cast<int64_t>(p.rows) * p.cols;
   const T* g = static_cast<const T*>(ins.u[b]);
+  float* mom = STEP ? ins.mom[b] : nullptr;
+  const float scale = STEP ? grad_factor(p) : 1.f;
   double s = 0.0;
+  auto one = [&](float gi, float& mi) {  // a value's square joins s; mi: momentum, updated
+    float u = gi;
+    if constexpr (STEP) {
+      gi *= scale;
+      mi = mi + (1.f - p.momentum) * (gi - mi);
+      u = p.nesterov ? gi + p.momentum * (mi - gi) : mi;
+    }
+    s += static_cast<double>(u) * u;
+  };
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kStartThreads;
-  if constexpr (STEP) {
-    float* mom = ins.mom[b];
-    const float scale = grad_factor(p);
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kStartThreads + threadIdx.x; i < n; i += stride) {
-      const float gi = to_f32(g[i]) * scale;
-      const float old = mom[i];
-      const float mi = old + (1.f - p.momentum) * (gi - old);
-      mom[i] = mi;
-      const float u = p.nesterov ? gi + p.momentum * (mi - gi) : mi;
-      s += static_cast<double>(u) * u;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kStartThreads + threadIdx.x;
+  int64_t done = 0;
+  if (aligned_for<T, STEP>(g, mom)) {  // four values at a time, two such loads under way
+    done = n & ~int64_t(3);
+    for (int64_t i = first; i < done / 4; i += 2 * stride) {
+      float v[2][4];
+      float4 o[2];
+      const bool two = i + stride < done / 4;
+      load4(g + 4 * i, v[0]);
+      if (two) load4(g + 4 * (i + stride), v[1]);
+      if constexpr (STEP) {
+        o[0] = reinterpret_cast<const float4*>(mom)[i];
+        if (two) o[1] = reinterpret_cast<const float4*>(mom)[i + stride];
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (k == 1 && !two) break;
+        one(v[k][0], o[k].x);
+        one(v[k][1], o[k].y);
+        one(v[k][2], o[k].z);
+        one(v[k][3], o[k].w);
+        if constexpr (STEP) reinterpret_cast<float4*>(mom)[i + k * stride] = o[k];
+      }
     }
-  } else {
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kStartThreads + threadIdx.x; i < n; i += stride) {
-      const double u = to_f32(g[i]);
-      s += u * u;
-    }
+  }
+  for (int64_t i = done + first; i < n; i += stride) {
+    float mi = STEP ? mom[i] : 0.f;
+    one(to_f32(g[i]), mi);
+    if constexpr (STEP) mom[i] = mi;
   }
   s = block_sum<kStartThreads>(s);
   if (threadIdx.x == 0) p.partial[b * p.parts + blockIdx.x] = s;
@@ -564,6 +689,8 @@ template <typename T, bool STEP>
 __global__ void __launch_bounds__(kStartThreads) ns_first_kernel(const __grid_constant__ Ins ins, const StartParams p) {
   __shared__ double factor_s;
   const int b = blockIdx.y;
+  pdl_launch();
+  pdl_wait();
   if (threadIdx.x < 32) {
     double s = 0.0;
     for (int i = threadIdx.x; i < p.parts; i += 32) s += p.partial[b * p.parts + i];
@@ -578,6 +705,7 @@ __global__ void __launch_bounds__(kStartThreads) ns_first_kernel(const __grid_co
   const T* g = static_cast<const T*>(ins.u[b]);
   const float* mom = STEP ? ins.mom[b] : nullptr;
   const float scale = STEP ? grad_factor(p) : 1.f;
+  const bool vec = p.cols % 4 == 0 && aligned_for<T, STEP>(g, mom);
   const int groups = p.ld / 8;
   const int64_t total = static_cast<int64_t>(p.rows) * groups;
   const int64_t base = static_cast<int64_t>(b) * p.rows * p.ld;
@@ -586,18 +714,34 @@ __global__ void __launch_bounds__(kStartThreads) ns_first_kernel(const __grid_co
     const int64_t r = i / groups;
     const int c = static_cast<int>(i - r * groups) * 8;
     float x[8];
+    auto value = [&](float u, float mi) {
+      if constexpr (STEP) {
+        u *= scale;
+        u = p.nesterov ? u + p.momentum * (mi - u) : mi;
+      }
+      return static_cast<float>(u * factor);
+    };
+    if (vec && c + 8 <= p.cols) {
+      const int64_t at = r * p.cols + c;
+      float v[2][4];
+      float4 o[2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[j] = 0.f;
-      if (c + j < p.cols) {
+      for (int k = 0; k < 2; ++k) {
+        load4(g + at + 4 * k, v[k]);
+        if constexpr (STEP) o[k] = *reinterpret_cast<const float4*>(mom + at + 4 * k);
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        x[4 * k] = value(v[k][0], o[k].x);
+        x[4 * k + 1] = value(v[k][1], o[k].y);
+        x[4 * k + 2] = value(v[k][2], o[k].z);
+        x[4 * k + 3] = value(v[k][3], o[k].w);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
         const int64_t at = r * p.cols + c + j;
-        float u = to_f32(g[at]);
-        if constexpr (STEP) {
-          u *= scale;
-          const float mi = mom[at];
-          u = p.nesterov ? u + p.momentum * (mi - u) : mi;
-        }
-        x[j] = static_cast<float>(u * factor);
+        x[j] = c + j < p.cols ? value(to_f32(g[at]), STEP ? mom[at] : 0.f) : 0.f;
       }
     }
     uint32_t h[4], l[4];
@@ -637,13 +781,15 @@ void product(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, cons
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = SMEM_BYTES;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, p, outs));
 }
 
@@ -783,8 +929,16 @@ template <typename T, bool STEP>
 void start(const Ins& ins, const StartParams& q, const Shape& s, int ctas, cudaStream_t stream) {
   ns_norm_kernel<T, STEP><<<dim3(q.parts, s.count), kStartThreads, 0, stream>>>(ins, q);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  ns_first_kernel<T, STEP><<<dim3(ctas, s.count), kStartThreads, 0, stream>>>(ins, q);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas, s.count);
+  cfg.blockDim = dim3(kStartThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, ns_first_kernel<T, STEP>, ins, q));
 }
 
 void check_sizes(int64_t rows, int64_t cols, int64_t steps, const std::vector<double>& coefficients) {
