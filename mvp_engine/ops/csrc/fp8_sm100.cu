@@ -115,11 +115,15 @@ struct Eight<float> {
 // One CTA per 128 x 128 tile.  Thread (g, l) holds rows 8 g .. 8 g + 7 of columns 8 l .. 8 l + 7: a row's 128 columns are
 // 16 lanes (its largest magnitude is four shuffles), and the 8 rows make 8-byte pieces of the transposed codes, which
 // go through shared memory (16-byte pieces swizzled by column group, free of bank conflicts) to leave as whole rows.
+// bf16 magnitudes are compared two at a time as 16-bit integers; that and four resident CTAs per SM (64 registers)
+// keep the kernel near memory speed.
 template <typename T, bool E5M2, bool TILE>
-__global__ void __launch_bounds__(QT) quantize_kernel(const QuantParams p) {
+__global__ void __launch_bounds__(QT, sizeof(T) == 2 ? 4 : 2) quantize_kernel(const QuantParams p) {
+  constexpr bool BF16 = sizeof(T) == 2;
   __shared__ __align__(16) uint8_t turned[BLOCK * BLOCK];
   __shared__ uint32_t col_max[QT / 32][BLOCK];
-  __shared__ int col_byte[BLOCK];
+  __shared__ __align__(16) float col_inv[BLOCK];  // 2^-e of each column's block; 0: it is not finite
+  __shared__ uint8_t col_byte[BLOCK];
   const int tile_r = blockIdx.x / p.tile_cols, tile_c = blockIdx.x - tile_r * p.tile_cols;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int l = threadIdx.x % 16, g = threadIdx.x / 16;
@@ -130,19 +134,25 @@ __global__ void __launch_bounds__(QT) quantize_kernel(const QuantParams p) {
     const int n = (r0 + i < p.rows) ? p.cols - c0 : 0;
     v[i].load(static_cast<const T*>(p.x) + static_cast<int64_t>(n > 0 ? r0 + i : 0) * p.ld + (n > 0 ? c0 : 0), n, p.vec);
   }
-  uint32_t row_max[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    uint32_t m = 0u;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, v[i].bits(j) & 0x7FFFFFFFu);
-    row_max[i] = m;
-  }
+  auto publish = [&](int col, uint32_t amax_bits) {
+    const int b = scale_byte<E5M2>(amax_bits);
+    col_inv[col] = b < 0 ? 0.f : inverse_scale(b);
+    col_byte[col] = static_cast<uint8_t>(b < 0 ? 127 : b);
+  };
   int row_b[8];
   if constexpr (TILE) {
     uint32_t m = 0u;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, row_max[i]);
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (BF16) {
+        m = __vmaxu2(m, __vmaxu2(__vmaxu2(v[i].u.x & 0x7FFF7FFFu, v[i].u.y & 0x7FFF7FFFu),
+                                 __vmaxu2(v[i].u.z & 0x7FFF7FFFu, v[i].u.w & 0x7FFF7FFFu)));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, v[i].bits(j) & 0x7FFFFFFFu);
+      }
+    }
+    if constexpr (BF16) m = max(m & 0xFFFF0000u, m << 16);
     m = __reduce_max_sync(0xffffffffu, m);
     if (lane == 0) col_max[warp][0] = m;
     __syncthreads();
@@ -151,32 +161,74 @@ __global__ void __launch_bounds__(QT) quantize_kernel(const QuantParams p) {
     const int b = scale_byte<E5M2>(m);
 #pragma unroll
     for (int i = 0; i < 8; ++i) row_b[i] = b;
-    if (threadIdx.x < BLOCK) col_byte[threadIdx.x] = b;
+    if (threadIdx.x < BLOCK) publish(threadIdx.x, m);
     __syncthreads();
   } else {
     if (p.q != nullptr) {
+      if constexpr (BF16) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+        for (int k = 0; k < 4; ++k) {  // rows 2 k (low half) and 2 k + 1 (high half)
+          uint32_t m[2];
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) row_max[i] = max(row_max[i], __shfl_xor_sync(0xffffffffu, row_max[i], o));
-        row_b[i] = scale_byte<E5M2>(row_max[i]);
+          for (int h = 0; h < 2; ++h) {
+            const uint4 u = v[2 * k + h].u;
+            m[h] = __vmaxu2(__vmaxu2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu), __vmaxu2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
+          }
+          uint32_t both = __vmaxu2(__byte_perm(m[0], m[1], 0x5410), __byte_perm(m[0], m[1], 0x7632));
+#pragma unroll
+          for (int o = 8; o > 0; o >>= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, o));
+          row_b[2 * k] = scale_byte<E5M2>(both << 16);
+          row_b[2 * k + 1] = scale_byte<E5M2>(both & 0xFFFF0000u);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t m = 0u;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) m = max(m, v[i].bits(j) & 0x7FFFFFFFu);
+#pragma unroll
+          for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+          row_b[i] = scale_byte<E5M2>(m);
+        }
       }
     }
     if (p.qt != nullptr) {
+      if constexpr (BF16) {
+        uint32_t m[4] = {0u, 0u, 0u, 0u};  // columns 8 l + 2 k (low half) and 8 l + 2 k + 1
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        uint32_t m = 0u;
+        for (int i = 0; i < 8; ++i) {
+          m[0] = __vmaxu2(m[0], v[i].u.x & 0x7FFF7FFFu);
+          m[1] = __vmaxu2(m[1], v[i].u.y & 0x7FFF7FFFu);
+          m[2] = __vmaxu2(m[2], v[i].u.z & 0x7FFF7FFFu);
+          m[3] = __vmaxu2(m[3], v[i].u.w & 0x7FFF7FFFu);
+        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, v[i].bits(j) & 0x7FFFFFFFu);
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 16));
-        if (lane < 16) col_max[warp][l * 8 + j] = m;
-      }
-      __syncthreads();
-      if (threadIdx.x < BLOCK) {
-        uint32_t m = 0u;
+        for (int k = 0; k < 4; ++k) m[k] = __vmaxu2(m[k], __shfl_xor_sync(0xffffffffu, m[k], 16));
+        if (lane < 16) *reinterpret_cast<uint4*>(&col_max[warp][l * 4]) = make_uint4(m[0], m[1], m[2], m[3]);
+        __syncthreads();
+        if (threadIdx.x < BLOCK / 2) {
+          uint32_t t = 0u;
 #pragma unroll
-        for (int w = 0; w < QT / 32; ++w) m = max(m, col_max[w][threadIdx.x]);
-        col_byte[threadIdx.x] = scale_byte<E5M2>(m);
+          for (int w = 0; w < QT / 32; ++w) t = __vmaxu2(t, col_max[w][threadIdx.x]);
+          publish(2 * threadIdx.x, t << 16);
+          publish(2 * threadIdx.x + 1, t & 0xFFFF0000u);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint32_t m = 0u;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) m = max(m, v[i].bits(j) & 0x7FFFFFFFu);
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, 16));
+          if (lane < 16) col_max[warp][l * 8 + j] = m;
+        }
+        __syncthreads();
+        if (threadIdx.x < BLOCK) {
+          uint32_t m = 0u;
+#pragma unroll
+          for (int w = 0; w < QT / 32; ++w) m = max(m, col_max[w][threadIdx.x]);
+          publish(threadIdx.x, m);
+        }
       }
       __syncthreads();
     }
@@ -208,24 +260,25 @@ __global__ void __launch_bounds__(QT) quantize_kernel(const QuantParams p) {
   }
   if (p.qt != nullptr) {
     const int groups = (row_blocks + 3) / 4;
+    const float4 inv0 = *reinterpret_cast<const float4*>(col_inv + l * 8);
+    const float4 inv1 = *reinterpret_cast<const float4*>(col_inv + l * 8 + 4);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int b = col_byte[l * 8 + j];
-      const float f = inverse_scale(max(b, 0));
+      const float f = j == 0 ? inv0.x : j == 1 ? inv0.y : j == 2 ? inv0.z : j == 3 ? inv0.w
+                    : j == 4 ? inv1.x : j == 5 ? inv1.y : j == 6 ? inv1.z : inv1.w;
       uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         w[i] = codes2<E5M2>(__uint_as_float(v[2 * i].bits(j)) * f, __uint_as_float(v[2 * i + 1].bits(j)) * f);
       uint2 out = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
-      if (b < 0) out = nan_codes(p.rows - r0);
+      if (f == 0.f) out = nan_codes(p.rows - r0);
       *reinterpret_cast<uint2*>(turned + (l * 8 + j) * BLOCK + (g ^ l) * 8) = out;
     }
     if (threadIdx.x < BLOCK) {
       const int col = tile_c * BLOCK + threadIdx.x;
-      const int b = col_byte[threadIdx.x];
       uint8_t* a = p.st + (static_cast<int64_t>(tile_c) * groups + tile_r / 4) * ATOM + (threadIdx.x % 32) * 16 +
                    (threadIdx.x / 32) * 4;
-      a[tile_r % 4] = col < p.cols ? static_cast<uint8_t>(b < 0 ? 127 : b) : 0;
+      a[tile_r % 4] = col < p.cols ? col_byte[threadIdx.x] : 0;
       if (tile_r == row_blocks - 1)
         for (int k = tile_r % 4 + 1; k < 4; ++k) a[k] = 0;
     }
