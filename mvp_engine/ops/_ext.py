@@ -26,7 +26,7 @@ KERNELS_PER_CALL = {
     "layernorm_fwd": 1, "layernorm_bwd": 3, "bias_gelu_fwd": 1, "bias_gelu_bwd": 2, "vision_rope_fwd": 1,
     "vision_rope_bwd": 1, "bias_residual_fwd": 1, "bias_grad": 2,
     "peer_gather_shards": 1, "publish_epoch": 1, "gemm_pair_gather": 1,
-    "quantize_fp8": 1, "gemm_fp8": 1,
+    "quantize_fp8": 1, "gemm_fp8": 1, "linear_fp8_fwd": 3, "linear_fp8_bwd": 3,
     "orthogonalize": 17, "muon_step_": 17,  # norm, first X and three products for each of five iterations
 }
 launch_count = 0
@@ -51,6 +51,7 @@ class _Counting:
                 launch_count += k
             return fn(*a, **kw)
 
+        self.__dict__[name] = wrapped  # found directly from now on
         return wrapped
 
 

@@ -111,11 +111,17 @@ void muon_step_(const std::vector<torch::Tensor>& p, const std::vector<torch::Te
                 double eps, double grad_scale, const c10::optional<torch::Tensor>& norm_sq, double max_norm,
                 int64_t status_ptr);
 
-void quantize_fp8(const torch::Tensor& x, bool tile, const c10::optional<torch::Tensor>& q,
-                  const c10::optional<torch::Tensor>& s, const c10::optional<torch::Tensor>& qt,
-                  const c10::optional<torch::Tensor>& st);
+std::vector<torch::Tensor> quantize_fp8(const torch::Tensor& x, bool tile, bool rows, bool columns, bool e5m2);
 void gemm_fp8(const torch::Tensor& a, const torch::Tensor& sa, const torch::Tensor& b, const torch::Tensor& sb,
-              torch::Tensor& c, bool accumulate, int64_t status_ptr);
+              int64_t cols, torch::Tensor& c, bool accumulate, int64_t status_ptr);
+std::vector<torch::Tensor> linear_fp8_fwd(const torch::Tensor& x, const torch::Tensor& w,
+                                          const c10::optional<torch::Tensor>& w8, const c10::optional<torch::Tensor>& sw8,
+                                          bool need_xt, bool need_wt, int64_t status_ptr);
+std::vector<torch::Tensor> linear_fp8_bwd(const torch::Tensor& dy, const c10::optional<torch::Tensor>& xt,
+                                          const c10::optional<torch::Tensor>& sxt,
+                                          const c10::optional<torch::Tensor>& wt,
+                                          const c10::optional<torch::Tensor>& swt, bool e5m2,
+                                          c10::optional<torch::Tensor> acc, int64_t status_ptr);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "mvp_engine sm_100a kernels";
@@ -175,5 +181,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("nesterov"), py::arg("steps"), py::arg("coefficients"), py::arg("eps"), py::arg("grad_scale"),
         py::arg("norm_sq"), py::arg("max_norm"), py::arg("status_ptr"));
   m.def("quantize_fp8", &quantize_fp8, "8-bit codes and block scales of a matrix's rows and / or columns");
+  m.def("linear_fp8_fwd", &linear_fp8_fwd, "quantise x and w, y = x w^T; keeps the transposed codes asked for");
+  m.def("linear_fp8_bwd", &linear_fp8_bwd, "quantise dy; dx = dy w and dw = dy^T x from kept codes");
   m.def("gemm_fp8", &gemm_fp8, "C (+)= A * B^T of 8-bit matrices with a scale per block of 128 (tcgen05 block-scaled)");
 }

@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(QT, sizeof(T) == 2 ? 4 : 2) quantize_kernel(co
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int l = threadIdx.x % 16, g = threadIdx.x / 16;
   const int r0 = tile_r * BLOCK + g * 8, c0 = tile_c * BLOCK + l * 8;
+  pdl_launch();
   Eight<T> v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -294,18 +295,25 @@ __global__ void __launch_bounds__(QT, sizeof(T) == 2 ? 4 : 2) quantize_kernel(co
         *reinterpret_cast<uint4*>(p.qt + (static_cast<int64_t>(tile_c) * BLOCK + col) * ldt + tile_r * BLOCK + k * 16) = u;
     }
   }
+  // Where this kernel may start before the one in front of it has ended (the second quantisation of a linear layer, which
+  // shares nothing with the first), it ends after it: what waits for this kernel may then rely on both.
+  pdl_wait();
 }
 
 template <typename T>
-void quantize(const QuantParams& p, bool e5m2, bool tile, int ctas, cudaStream_t stream) {
-  if (tile) {
-    if (e5m2) quantize_kernel<T, true, true><<<ctas, QT, 0, stream>>>(p);
-    else quantize_kernel<T, false, true><<<ctas, QT, 0, stream>>>(p);
-  } else {
-    if (e5m2) quantize_kernel<T, true, false><<<ctas, QT, 0, stream>>>(p);
-    else quantize_kernel<T, false, false><<<ctas, QT, 0, stream>>>(p);
-  }
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+void quantize(const QuantParams& p, bool e5m2, bool tile, int ctas, bool early, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(QT);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = early ? 1 : 0;
+  auto kern = tile ? (e5m2 ? quantize_kernel<T, true, true> : quantize_kernel<T, false, true>)
+                   : (e5m2 ? quantize_kernel<T, true, false> : quantize_kernel<T, false, false>);
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, p));
 }
 
 }  // namespace fp8
@@ -314,32 +322,46 @@ void quantize(const QuantParams& p, bool e5m2, bool tile, int ctas, cudaStream_t
 //   C[M, N] (+)= A[M, K] B[N, K]^T of two such matrices, fp32 accumulation
 //
 // The pair-of-SMs GEMM (roles as in gemm2sm_sm100.cu) with tcgen05.mma kind::mxf8f6f4.block_scale: per 128-deep
-// k-block each CTA loads 128 rows of A and of B (16 KB each) and every fourth k-block three scale atoms (its 128 rows
-// of A; all 256 rows of B, which both SMs of a pair need), which tcgen05.cp moves to tensor memory; the
+// k-block each CTA loads 128 rows of A and half a tile's rows of B and every fourth k-block the scale atoms (its 128 rows
+// of A; all rows of B, which both SMs of a pair need), which tcgen05.cp moves to tensor memory; the
 // k-block's byte of a scale word is picked by the instruction descriptor.
-// Tensor memory: two 256-column accumulators at columns 0 and 192 share 64 columns, because the last 64 hold four
-// sets of scales (16 columns each).  The epilogue reads the shared columns of a tile first and hands them back at
-// once, so the next tile's MMAs wait only for that.  A set is reused four groups (16 k-blocks) later; the ring has 6
-// stages, so a full stage there means that the group's MMAs are done, and a tile starts only after the last one's.
+//
+// Tiles are 256 x TN, TN = 256, 192 or 128, whichever gives the shortest schedule (choose_tile).
+// Tensor memory: the last 64 of 512 columns hold four sets of scales (16 columns each); the accumulators start at
+// columns 0 and 192.  For TN = 256 they share 64 columns: the epilogue reads those first and hands them back at
+// once, and the next tile's MMAs wait for that.  For smaller tiles they wait only for the tile two before.
+// A set of scales is used again four groups (of four k-blocks) later.  At most one tile boundary lies in between (the
+// tile two before has been read out), so at least 10 k-blocks do, more than the ring's stages: the full
+// stage that the new group waits for was emptied after the old group's MMAs.
 namespace fp8gemm {
 
 using namespace gemm2;
 using fp8::ATOM;
 
 constexpr int BK = 128;
-constexpr int TILE = 256;
+constexpr int TM = 256;
 constexpr int HALF = 128;
-constexpr int STAGES = 6;
-constexpr int OP_BYTES = HALF * BK;
-constexpr int SF_BYTES = 3 * ATOM;
-constexpr int STAGE_BYTES = 2 * OP_BYTES;
+constexpr int A_BYTES = HALF * BK;
 constexpr int TMEM_COLS = 512;
-constexpr int ACC1_COL = 192;  // accumulator 0: columns 0..255, accumulator 1: 192..447
+constexpr int ACC1_COL = 192;
 constexpr int SF_COL = 448;
-constexpr int THREADS = 192;
-constexpr int SMEM_BYTES = STAGES * (STAGE_BYTES + SF_BYTES) + 1024 + 256;
+constexpr int EPI_WARPS = 8;  // two for each quarter of the accumulator's lanes, half of the columns each
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int CHUNK = 32;     // columns the epilogue handles at a time
 
 enum Epilogue : int { kStoreBf16 = 0, kStoreF32 = 1, kAccumF32 = 2 };
+
+template <int TN, int EPI>
+struct Plan {
+  static constexpr int B_BYTES = TN / 2 * BK;
+  static constexpr int SFB = TN == 128 ? 1 : 2;  // atoms that TN columns touch (192: 64 columns off every other tile)
+  static constexpr int SF_BYTES = (1 + SFB) * ATOM;
+  static constexpr int STAGES = EPI == kStoreBf16 ? 6 : 5;
+  static constexpr int EPI_BUF = 32 * CHUNK * (EPI == kStoreBf16 ? 2 : 4);
+  static constexpr int SMEM = STAGES * (A_BYTES + B_BYTES + SF_BYTES) + EPI_WARPS * EPI_BUF + 1024 + 256;
+  static constexpr bool SHARED_COLS = TN > ACC1_COL;
+  static constexpr int CHUNKS = TN / 2 / CHUNK;  // per epilogue warp
+};
 
 struct Params {
   int M, N;
@@ -347,6 +369,7 @@ struct Params {
   int sf_groups;  // scale atoms per 128 rows
   void* C;
   int64_t ldc;
+  bool vec;     // rows of C are 16-byte aligned
   uint32_t idesc;
   int* status;
 };
@@ -371,14 +394,15 @@ __device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint32_t smem_add
 
 // kind::mxf8f6f4: types (0 e4m3, 1 e5m2) at bits 7 and 10, N / 8 at 17, unsigned-exponent scales at 23, M / 16 at 24;
 // the scale byte of the k-block goes to bits 29 (A) and 4 (B).
-inline uint32_t make_idesc(bool a_e5m2, bool b_e5m2) {
-  return ((a_e5m2 ? 1u : 0u) << 7) | ((b_e5m2 ? 1u : 0u) << 10) | ((static_cast<uint32_t>(TILE) >> 3) << 17) |
-         (1u << 23) | ((static_cast<uint32_t>(TILE) >> 4) << 24);
+inline uint32_t make_idesc(bool a_e5m2, bool b_e5m2, int tn) {
+  return ((a_e5m2 ? 1u : 0u) << 7) | ((b_e5m2 ? 1u : 0u) << 10) | ((static_cast<uint32_t>(tn) >> 3) << 17) |
+         (1u << 23) | ((static_cast<uint32_t>(TM) >> 4) << 24);
 }
 
+template <int TN>
 __device__ __forceinline__ void tile_coords(const Params& p, int t, int& tm, int& tn) {
   constexpr int kGroup = 8;
-  const int num_m = (p.M + TILE - 1) / TILE, num_n = (p.N + TILE - 1) / TILE;
+  const int num_m = (p.M + TM - 1) / TM, num_n = (p.N + TN - 1) / TN;
   const int per_group = kGroup * num_n;
   const int g = t / per_group, first = g * kGroup;
   const int gm = min(kGroup, num_m - first);
@@ -387,63 +411,96 @@ __device__ __forceinline__ void tile_coords(const Params& p, int t, int& tm, int
   tn = r / gm;
 }
 
+// A warp's 32 rows x 32 columns from one row per lane to C: through the warp's shared memory in 16-byte pieces swizzled by
+// row, so that 4 (bf16) or 8 (fp32) consecutive lanes write each row.
 template <int EPI>
-__device__ __forceinline__ void store_chunk(const Params& p, int m, int n, const uint32_t (&r)[32]) {
-  if (m >= p.M || n >= p.N) return;
-  const bool full = n + 32 <= p.N;
+__device__ __forceinline__ void store_chunk(const Params& p, uint8_t* buf, int m0, int n, const uint32_t (&r)[32]) {
+  if (m0 >= p.M || n >= p.N) return;  // same for all lanes
+  const int lane = threadIdx.x % 32;
   if constexpr (EPI == kStoreBf16) {
-    __nv_bfloat16* C = static_cast<__nv_bfloat16*>(p.C) + static_cast<int64_t>(m) * p.ldc + n;
-    if (full && (reinterpret_cast<uintptr_t>(C) & 15) == 0) {
+    auto piece = [](int row, int j) { return row * 64 + ((j ^ ((row >> 1) & 3)) << 4); };
 #pragma unroll
-      for (int v = 0; v < 4; ++v)
-        reinterpret_cast<uint4*>(C)[v] =
-            make_uint4(pack_bf16x2(__uint_as_float(r[8 * v]), __uint_as_float(r[8 * v + 1])),
-                       pack_bf16x2(__uint_as_float(r[8 * v + 2]), __uint_as_float(r[8 * v + 3])),
-                       pack_bf16x2(__uint_as_float(r[8 * v + 4]), __uint_as_float(r[8 * v + 5])),
-                       pack_bf16x2(__uint_as_float(r[8 * v + 6]), __uint_as_float(r[8 * v + 7])));
-    } else {
+    for (int v = 0; v < 4; ++v)
+      *reinterpret_cast<uint4*>(buf + piece(lane, v)) =
+          make_uint4(pack_bf16x2(__uint_as_float(r[8 * v]), __uint_as_float(r[8 * v + 1])),
+                     pack_bf16x2(__uint_as_float(r[8 * v + 2]), __uint_as_float(r[8 * v + 3])),
+                     pack_bf16x2(__uint_as_float(r[8 * v + 4]), __uint_as_float(r[8 * v + 5])),
+                     pack_bf16x2(__uint_as_float(r[8 * v + 6]), __uint_as_float(r[8 * v + 7])));
+    __syncwarp();
+    __nv_bfloat16* C = static_cast<__nv_bfloat16*>(p.C) + static_cast<int64_t>(m0) * p.ldc + n;
+    if (p.vec && n + CHUNK <= p.N) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (n + j < p.N) C[j] = __float2bfloat16_rn(__uint_as_float(r[j]));
-    }
-  } else {
-    float* C = static_cast<float*>(p.C) + static_cast<int64_t>(m) * p.ldc + n;
-    if (full && (reinterpret_cast<uintptr_t>(C) & 15) == 0) {
-#pragma unroll
-      for (int v = 0; v < 8; ++v) {
-        float4 q = make_float4(__uint_as_float(r[4 * v]), __uint_as_float(r[4 * v + 1]), __uint_as_float(r[4 * v + 2]),
-                               __uint_as_float(r[4 * v + 3]));
-        if constexpr (EPI == kAccumF32) {
-          const float4 o = reinterpret_cast<const float4*>(C)[v];
-          q.x += o.x;
-          q.y += o.y;
-          q.z += o.z;
-          q.w += o.w;
-        }
-        reinterpret_cast<float4*>(C)[v] = q;
+      for (int i = 0; i < 4; ++i) {
+        const int row = i * 8 + lane / 4, j = lane & 3;
+        if (m0 + row < p.M)
+          *reinterpret_cast<uint4*>(C + row * p.ldc + j * 8) = *reinterpret_cast<const uint4*>(buf + piece(row, j));
       }
     } else {
+#pragma unroll 8
+      for (int row = 0; row < 32; ++row)
+        if (m0 + row < p.M && n + lane < p.N)
+          C[row * p.ldc + lane] = *reinterpret_cast<const __nv_bfloat16*>(buf + piece(row, lane / 8) + (lane & 7) * 2);
+    }
+  } else {
+    auto piece = [](int row, int j) { return row * 128 + ((j ^ (row & 7)) << 4); };
+    float* C = static_cast<float*>(p.C) + static_cast<int64_t>(m0) * p.ldc + n;
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (n + j < p.N) C[j] = __uint_as_float(r[j]) + (EPI == kAccumF32 ? C[j] : 0.f);
+    for (int v = 0; v < 8; ++v)
+      *reinterpret_cast<uint4*>(buf + piece(lane, v)) = make_uint4(r[4 * v], r[4 * v + 1], r[4 * v + 2], r[4 * v + 3]);
+    __syncwarp();
+    if (p.vec && n + CHUNK <= p.N) {
+      const int j = lane & 7;
+#pragma unroll
+      for (int i0 = 0; i0 < 8; i0 += 4) {
+        float4 o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (EPI == kAccumF32 && m0 + (i0 + i) * 4 + lane / 8 < p.M)
+            o[i] = *reinterpret_cast<const float4*>(C + ((i0 + i) * 4 + lane / 8) * p.ldc + j * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = (i0 + i) * 4 + lane / 8;
+          if (m0 + row >= p.M) continue;
+          float4 q = *reinterpret_cast<const float4*>(buf + piece(row, j));
+          if constexpr (EPI == kAccumF32) {
+            q.x += o[i].x;
+            q.y += o[i].y;
+            q.z += o[i].z;
+            q.w += o[i].w;
+          }
+          *reinterpret_cast<float4*>(C + row * p.ldc + j * 4) = q;
+        }
+      }
+    } else {
+#pragma unroll 4
+      for (int row = 0; row < 32; ++row)
+        if (m0 + row < p.M && n + lane < p.N) {
+          float q = *reinterpret_cast<const float*>(buf + piece(row, lane / 4) + (lane & 3) * 4);
+          if constexpr (EPI == kAccumF32) q += C[row * p.ldc + lane];
+          C[row * p.ldc + lane] = q;
+        }
     }
   }
+  __syncwarp();  // the buffer may be written again
 }
 
-template <int EPI>
+template <int TN, int EPI>
 __global__ void __launch_bounds__(THREADS, 1)
     fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB, const Params p) {
+  using P = Plan<TN, EPI>;
+  constexpr int STAGES = P::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
-  uint8_t* sB = smem + STAGES * OP_BYTES;
-  uint8_t* sS = smem + STAGES * STAGE_BYTES;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sS + STAGES * SF_BYTES);  // used in the leader
-  uint64_t* empty_bar = full_bar + STAGES;                                   // both CTAs
-  uint64_t* tfull_bar = empty_bar + STAGES;                                  // [2] both CTAs
-  uint64_t* handed_bar = tfull_bar + 2;                                      // used in the leader: shared columns read
-  uint64_t* done_bar = handed_bar + 1;
+  uint8_t* sB = smem + STAGES * A_BYTES;
+  uint8_t* sS = sB + STAGES * P::B_BYTES;
+  uint8_t* sE = sS + STAGES * P::SF_BYTES;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sE + EPI_WARPS * P::EPI_BUF);  // used in the leader
+  uint64_t* empty_bar = full_bar + STAGES;                                        // both CTAs
+  uint64_t* tfull_bar = empty_bar + STAGES;                                       // [2] both CTAs
+  uint64_t* handed_bar = tfull_bar + 2;  // [2] used in the leader: an accumulator (or its shared columns) has been read
+  uint64_t* done_bar = handed_bar + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -452,15 +509,17 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t crank = cluster_ctarank();  // 0 = leader
   const int cluster_id = blockIdx.x >> 1;
   const int clusters = gridDim.x >> 1;
-  const int total = ((p.M + TILE - 1) / TILE) * ((p.N + TILE - 1) / TILE);
+  const int total = ((p.M + TM - 1) / TM) * ((p.N + TN - 1) / TN);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
-    for (int a = 0; a < 2; ++a) mbar_init(&tfull_bar[a], 1);
-    mbar_init(handed_bar, 2 * 128);  // epilogue threads of both CTAs
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull_bar[a], 1);
+      mbar_init(&handed_bar[a], 2 * 32 * EPI_WARPS);  // epilogue threads of both CTAs
+    }
     mbar_init(done_bar, 1);
     *abort_flag = 0;
     fence_mbarrier_init();
@@ -479,6 +538,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   cluster_sync_all();  // barriers of both CTAs initialised before any remote arrive / copy
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  pdl_launch();
+  pdl_wait();  // every thread: the operands are written by the kernels before this one
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer (both CTAs)
@@ -489,25 +550,27 @@ __global__ void __launch_bounds__(THREADS, 1)
       bool ok = true, issued = false;
       for (int t = cluster_id; ok && t < total; t += clusters) {
         int tm, tn;
-        tile_coords(p, t, tm, tn);
-        const int m0 = tm * TILE + crank * HALF, n0 = tn * TILE + crank * HALF;
-        const int sa = (tm * 2 + static_cast<int>(crank)) * p.sf_groups, sb = tn * 2 * p.sf_groups;
+        tile_coords<TN>(p, t, tm, tn);
+        const int m0 = tm * TM + crank * HALF, n0 = tn * TN + crank * (TN / 2);
+        const int sa = (tm * 2 + static_cast<int>(crank)) * p.sf_groups, sb = (tn * TN / HALF) * p.sf_groups;
         for (int kb = 0; kb < p.num_kb; ++kb) {
           if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1, abort_flag, p.status, kTimeoutProducer)) {
             ok = false;
             break;
           }
           const bool scales = (kb & 3) == 0;
-          if (crank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * (STAGE_BYTES + (scales ? SF_BYTES : 0)));
+          if (crank == 0)
+            mbar_arrive_expect_tx(&full_bar[stage], 2 * (A_BYTES + P::B_BYTES + (scales ? P::SF_BYTES : 0)));
           issued = true;
           const uint32_t bar = leader_full0 + stage * 8;
-          tma_load_2d_pair(sA + stage * OP_BYTES, &tmA, bar, kb * BK, m0);
-          tma_load_2d_pair(sB + stage * OP_BYTES, &tmB, bar, kb * BK, n0);
+          tma_load_2d_pair(sA + stage * A_BYTES, &tmA, bar, kb * BK, m0);
+          tma_load_2d_pair(sB + stage * P::B_BYTES, &tmB, bar, kb * BK, n0);
           if (scales) {
-            uint8_t* dst = sS + stage * SF_BYTES;
+            uint8_t* dst = sS + stage * P::SF_BYTES;
             tma_load_2d_pair(dst, &tmSA, bar, 0, sa + kb / 4);
-            tma_load_2d_pair(dst + ATOM, &tmSB, bar, 0, sb + kb / 4);
-            tma_load_2d_pair(dst + 2 * ATOM, &tmSB, bar, 0, sb + p.sf_groups + kb / 4);
+#pragma unroll
+            for (int a = 0; a < P::SFB; ++a)
+              tma_load_2d_pair(dst + (1 + a) * ATOM, &tmSB, bar, 0, sb + a * p.sf_groups + kb / 4);
           }
           if (++stage == STAGES) {
             stage = 0;
@@ -530,12 +593,15 @@ __global__ void __launch_bounds__(THREADS, 1)
       int local = 0, group = 0;
       bool ok = true;
       for (int t = cluster_id; ok && t < total; t += clusters, ++local) {
-        // the columns this tile shares with the one before have been read (completion number `local`)
-        if (local > 0 &&
-            !mbar_wait_bounded(handed_bar, (local - 1) & 1, abort_flag, p.status, kTimeoutMma))
+        const int before = local - (P::SHARED_COLS ? 1 : 2);  // the tile whose read-out this one waits for
+        if (before >= 0 &&
+            !mbar_wait_bounded(&handed_bar[before & 1], (before >> 1) & 1, abort_flag, p.status, kTimeoutMma))
           break;
         tc_fence_after();
+        int tm, tn;
+        tile_coords<TN>(p, t, tm, tn);
         const uint32_t d_tmem = tmem_base + (local & 1) * ACC1_COL;
+        const uint32_t shift = (tn * TN % HALF) / 32;  // TN = 192: an odd tile starts at row 64 of its first atom
         uint32_t sf = 0;
         for (int kb = 0; kb < p.num_kb; ++kb) {
           if (!mbar_wait_bounded(&full_bar[stage], phase, abort_flag, p.status, kTimeoutMma)) {
@@ -545,18 +611,18 @@ __global__ void __launch_bounds__(THREADS, 1)
           tc_fence_after();
           if ((kb & 3) == 0) {
             sf = tmem_base + SF_COL + (group++ & 3) * 16;
-            const uint32_t src = smem_u32(sS + stage * SF_BYTES);
+            const uint32_t src = smem_u32(sS + stage * P::SF_BYTES);
             scales_to_tmem(sf, src);
-            scales_to_tmem(sf + 8, src + ATOM);
-            scales_to_tmem(sf + 12, src + 2 * ATOM);
+#pragma unroll
+            for (int a = 0; a < P::SFB; ++a) scales_to_tmem(sf + 8 + 4 * a, src + (1 + a) * ATOM);
           }
           const uint32_t idesc = p.idesc | (static_cast<uint32_t>(kb & 3) << 29) | (static_cast<uint32_t>(kb & 3) << 4);
-          const uint32_t a_base = smem_u32(sA + stage * OP_BYTES);
-          const uint32_t b_base = smem_u32(sB + stage * OP_BYTES);
+          const uint32_t a_base = smem_u32(sA + stage * A_BYTES);
+          const uint32_t b_base = smem_u32(sB + stage * P::B_BYTES);
 #pragma unroll
           for (int k = 0; k < BK / 32; ++k)
             mma_scaled_pair(d_tmem, make_smem_desc_sw128(a_base + k * 32, 16, 1024),
-                            make_smem_desc_sw128(b_base + k * 32, 16, 1024), idesc, sf, sf + 8,
+                            make_smem_desc_sw128(b_base + k * 32, 16, 1024), idesc, sf, sf + 8 + shift,
                             (kb != 0 || k != 0) ? 1u : 0u);
           mma_commit_pair(&empty_bar[stage]);
           if (++stage == STAGES) {
@@ -572,40 +638,54 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs)
-    const int sub = warp & 3;
-    const int row_in_tile = crank * HALF + sub * 32 + lane;
-    const uint32_t leader_handed = mapa_shared(smem_u32(handed_bar), 0);
+    const int sub = warp & 3, ew = warp - 2, half = ew / 4;
+    uint8_t* const buf = sE + ew * P::EPI_BUF;
+    const uint32_t leader_handed = mapa_shared(smem_u32(&handed_bar[0]), 0);
     const uint32_t lanes = static_cast<uint32_t>(sub * 32) << 16;
     int local = 0;
     for (int t = cluster_id; t < total; t += clusters, ++local) {
       int tm, tn;
-      tile_coords(p, t, tm, tn);
+      tile_coords<TN>(p, t, tm, tn);
       const int acc = local & 1;
       if (!__all_sync(0xffffffffu, mbar_wait_bounded(&tfull_bar[acc], (local >> 1) & 1, abort_flag, p.status,
                                                      kTimeoutEpilogue)))
         break;
       tc_fence_after();
-      const int m = tm * TILE + row_in_tile;
-      const uint32_t base = tmem_base + lanes + acc * ACC1_COL;
-      // columns shared with the other accumulator: the last 64 of accumulator 0, the first 64 of accumulator 1
-      const int c_first = acc == 0 ? 6 : 0;
-      {
-        uint32_t r0[32], r1[32];
-        tmem_ld_32x32b_x32(base + c_first * 32, r0);
-        tmem_ld_32x32b_x32(base + c_first * 32 + 32, r1);
-        tmem_wait_ld();
-        tc_fence_before();
-        remote_arrive(leader_handed);
-        store_chunk<EPI>(p, m, tn * TILE + c_first * 32, r0);
-        store_chunk<EPI>(p, m, tn * TILE + c_first * 32 + 32, r1);
+      const int m0 = tm * TM + static_cast<int>(crank) * HALF + sub * 32;
+      const int n0 = tn * TN + half * (TN / 2);
+      const uint32_t base = tmem_base + lanes + acc * ACC1_COL + half * (TN / 2);
+      int first = 0, count = P::CHUNKS;  // chunks still to be read after the shared columns
+      if constexpr (P::SHARED_COLS) {
+        // columns shared with the other accumulator: the last 64 of accumulator 0, the first 64 of accumulator 1
+        const bool mine = half == 1 - acc;
+        if (mine) {
+          const int c = acc == 0 ? P::CHUNKS - 2 : 0;
+          uint32_t r0[32], r1[32];
+          tmem_ld_32x32b_x32(base + c * CHUNK, r0);
+          tmem_ld_32x32b_x32(base + c * CHUNK + CHUNK, r1);
+          tmem_wait_ld();
+          tc_fence_before();
+          remote_arrive(leader_handed + acc * 8);
+          store_chunk<EPI>(p, buf, m0, n0 + c * CHUNK, r0);
+          store_chunk<EPI>(p, buf, m0, n0 + c * CHUNK + CHUNK, r1);
+          first = acc == 0 ? 0 : 2;
+          count = P::CHUNKS - 2;
+        } else {
+          tc_fence_before();
+          remote_arrive(leader_handed + acc * 8);  // this warp's part of the tile before has been read
+        }
       }
 #pragma unroll 1
-      for (int i = 0; i < 6; ++i) {
-        const int c = acc == 0 ? i : i + 2;
+      for (int i = 0; i < count; ++i) {
+        const int c = first + i;
         uint32_t r[32];
-        tmem_ld_32x32b_x32(base + c * 32, r);
+        tmem_ld_32x32b_x32(base + c * CHUNK, r);
         tmem_wait_ld();
-        store_chunk<EPI>(p, m, tn * TILE + c * 32, r);
+        if (!P::SHARED_COLS && i == count - 1) {
+          tc_fence_before();
+          remote_arrive(leader_handed + acc * 8);
+        }
+        store_chunk<EPI>(p, buf, m0, n0 + c * CHUNK, r);
       }
     }
   }
@@ -633,61 +713,137 @@ inline void encode(CUtensorMap* map, CUtensorMapDataType type, const void* base,
   TORCH_CHECK(r == CUDA_SUCCESS, "gemm_fp8: cuTensorMapEncodeTiled failed with code ", static_cast<int>(r));
 }
 
-template <int EPI>
+// Tile width with the shortest schedule: waves x (cycles of a tile: its k-blocks, plus what it costs besides), and the last
+// tile's read-out.  A k-block of 128 takes 2 TN cycles at the tensor core's rate and a little more where A's share of the
+// shared-memory traffic grows.  Measured: 8192 x 4096 -> 24576 in 562 us with 192 columns, 600 with 256 (the hand-over
+// of the shared columns); 8192 x 4096 -> 4096 in 99 us with 256 (7 waves) and 153 with 128 (14 waves).
+inline int choose_tile(int64_t M, int64_t N, int num_kb, int sms) {
+  const int64_t clusters = std::max(1, sms / 2);
+  struct Width {
+    int tn, block, besides;
+  };
+  int best = 256;
+  int64_t best_cost = -1;
+  for (const Width w : {Width{256, 512, 700}, Width{192, 390, 150}, Width{128, 350, 150}}) {
+    const int64_t tiles = (M + TM - 1) / TM * ((N + w.tn - 1) / w.tn);
+    const int64_t waves = (tiles + clusters - 1) / clusters;
+    const int64_t cost = waves * (static_cast<int64_t>(w.block) * num_kb + w.besides) + 8 * w.tn;
+    if (best_cost < 0 || cost < best_cost) {
+      best = w.tn;
+      best_cost = cost;
+    }
+  }
+  return best;
+}
+
+template <int TN, int EPI>
 void launch(const CUtensorMap (&t)[4], const Params& p, int sms, cudaStream_t stream) {
-  auto kern = fp8_gemm_kernel<EPI>;
+  auto kern = fp8_gemm_kernel<TN, EPI>;
   static std::atomic<uint64_t> configured{0};
-  allow_smem(kern, SMEM_BYTES, configured);
-  const int64_t tiles = static_cast<int64_t>((p.M + TILE - 1) / TILE) * ((p.N + TILE - 1) / TILE);
+  allow_smem(kern, Plan<TN, EPI>::SMEM, configured);
+  const int64_t tiles = static_cast<int64_t>((p.M + TM - 1) / TM) * ((p.N + TN - 1) / TN);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * static_cast<unsigned>(std::min<int64_t>(tiles, std::max(1, sms / 2))));
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.dynamicSmemBytes = Plan<TN, EPI>::SMEM;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, t[0], t[1], t[2], t[3], p));
+}
+
+template <int TN>
+void launch_tile(int epi, const CUtensorMap (&t)[4], const Params& p, int sms, cudaStream_t stream) {
+  if (epi == kStoreBf16) launch<TN, kStoreBf16>(t, p, sms, stream);
+  else if (epi == kStoreF32) launch<TN, kStoreF32>(t, p, sms, stream);
+  else launch<TN, kAccumF32>(t, p, sms, stream);
 }
 
 }  // namespace fp8gemm
 }  // namespace mvp
 
-static bool is_e5m2(const torch::Tensor& t, const char* what) {
+namespace {
+
+using mvp::fp8::ATOM;
+using mvp::fp8::BLOCK;
+
+bool is_e5m2(const torch::Tensor& t, const char* what) {
   TORCH_CHECK(t.scalar_type() == at::kFloat8_e4m3fn || t.scalar_type() == at::kFloat8_e5m2, what,
               ": codes are float8_e4m3fn or float8_e5m2");
   return t.scalar_type() == at::kFloat8_e5m2;
 }
 
-// Codes and scale atoms of x's rows (q, s) and / or columns (qt, st); tile: 128 x 128 blocks instead of 1 x 128.
-void quantize_fp8(const torch::Tensor& x, bool tile, const c10::optional<torch::Tensor>& q,
-                  const c10::optional<torch::Tensor>& s, const c10::optional<torch::Tensor>& qt,
-                  const c10::optional<torch::Tensor>& st) {
-  using namespace mvp::fp8;
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.size(0) > 0 && x.size(1) > 0 && (x.stride(1) == 1 || x.size(1) == 1),
-              "quantize_fp8: CUDA matrix with unit column stride");
-  TORCH_CHECK(x.size(0) < (int64_t(1) << 31) - 256 && x.size(1) < (int64_t(1) << 31) - 256, "quantize_fp8: sizes");
-  const int64_t rb = (x.size(0) + BLOCK - 1) / BLOCK, cb = (x.size(1) + BLOCK - 1) / BLOCK;
-  TORCH_CHECK(rb * cb < (int64_t(1) << 31), "quantize_fp8: too many blocks");
+int64_t blocks_of(int64_t n) { return (n + BLOCK - 1) / BLOCK; }
+int64_t code_bytes(int64_t rows, int64_t cols) { return rows * blocks_of(cols) * BLOCK; }
+int64_t scale_bytes(int64_t rows, int64_t cols) { return blocks_of(rows) * ((blocks_of(cols) + 3) / 4) * ATOM; }
+
+// A quantised matrix [rows, cols] (or none: data == nullptr).
+struct Matrix {
+  uint8_t* data = nullptr;
+  uint8_t* scale = nullptr;
+  int64_t rows = 0, cols = 0;
   bool e5m2 = false;
-  auto check = [&](const c10::optional<torch::Tensor>& d, const c10::optional<torch::Tensor>& a, int64_t rows,
-                   int64_t blocks, int64_t row_blocks) {
-    if (!d.has_value()) return;
-    e5m2 = is_e5m2(*d, "quantize_fp8");
-    TORCH_CHECK(d->device() == x.device() && d->is_contiguous() && d->dim() == 2 && d->size(0) == rows &&
-                    d->size(1) == blocks * BLOCK && a.has_value() && a->device() == x.device() && a->is_contiguous() &&
-                    a->scalar_type() == at::kByte && a->numel() == row_blocks * ((blocks + 3) / 4) * ATOM,
-                "quantize_fp8: outputs");
-  };
-  check(q, s, x.size(0), cb, rb);
-  check(qt, st, x.size(1), rb, cb);
-  TORCH_CHECK(q.has_value() || qt.has_value(), "quantize_fp8: nothing to write");
-  TORCH_CHECK(!q.has_value() || !qt.has_value() || q->scalar_type() == qt->scalar_type(), "quantize_fp8: one type");
-  const at::cuda::CUDAGuard guard(x.device());
+};
+
+// The matrix of an Fp8Matrix's two tensors, checked.
+Matrix as_matrix(const torch::Tensor& data, const torch::Tensor& scale, int64_t cols, const torch::Device& dev,
+                 const char* what) {
+  Matrix m;
+  m.e5m2 = is_e5m2(data, what);
+  m.rows = data.size(0);
+  m.cols = cols;
+  TORCH_CHECK(data.device() == dev && data.dim() == 2 && data.is_contiguous() && data.size(0) > 0 && cols > 0 &&
+                  data.size(1) == blocks_of(cols) * BLOCK,
+              what, ": contiguous codes [rows, whole blocks of 128] on the operands' device");
+  TORCH_CHECK(scale.device() == dev && scale.scalar_type() == at::kByte && scale.is_contiguous() &&
+                  scale.numel() == scale_bytes(m.rows, cols),
+              what, ": scale bytes");
+  m.data = static_cast<uint8_t*>(data.data_ptr());
+  m.scale = scale.data_ptr<uint8_t>();
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(m.data) & 15) == 0 && (reinterpret_cast<uintptr_t>(m.scale) & 15) == 0, what,
+              ": 16-byte aligned codes and scales");
+  return m;
+}
+
+// New tensors for a quantised matrix.
+Matrix new_matrix(int64_t rows, int64_t cols, bool e5m2, const torch::Tensor& like, torch::Tensor& data,
+                  torch::Tensor& scale) {
+  data = torch::empty({rows, blocks_of(cols) * BLOCK}, like.options().dtype(e5m2 ? at::kFloat8_e5m2 : at::kFloat8_e4m3fn));
+  scale = torch::empty({blocks_of(rows), (blocks_of(cols) + 3) / 4, 32, 4, 4}, like.options().dtype(at::kByte));
+  Matrix m;
+  m.data = static_cast<uint8_t*>(data.data_ptr());
+  m.scale = scale.data_ptr<uint8_t>();
+  m.rows = rows;
+  m.cols = cols;
+  m.e5m2 = e5m2;
+  return m;
+}
+
+// Space in a call's own buffer for a matrix that does not outlive the call; `used` grows by it.
+void place(Matrix& m, int64_t rows, int64_t cols, bool e5m2, uint8_t* base, int64_t& used) {
+  auto up = [](int64_t n) { return (n + 511) / 512 * 512; };
+  m.rows = rows;
+  m.cols = cols;
+  m.e5m2 = e5m2;
+  m.data = base + used;
+  m.scale = m.data + up(code_bytes(rows, cols));
+  used += up(code_bytes(rows, cols)) + up(scale_bytes(rows, cols));
+}
+
+// x (checked: a CUDA matrix with unit column stride, bf16 or fp32) into q and / or, transposed, t.
+void quantize_into(const torch::Tensor& x, bool tile, const Matrix& q, const Matrix& t, bool early, cudaStream_t stream) {
+  using namespace mvp::fp8;
+  const int64_t rb = blocks_of(x.size(0)), cb = blocks_of(x.size(1));
+  TORCH_CHECK(x.size(0) < (int64_t(1) << 31) - 256 && x.size(1) < (int64_t(1) << 31) - 256 &&
+                  rb * cb < (int64_t(1) << 31),
+              "quantize_fp8: too many blocks");
   QuantParams p{};
   p.x = x.data_ptr();
   p.ld = x.stride(0);
@@ -695,72 +851,152 @@ void quantize_fp8(const torch::Tensor& x, bool tile, const c10::optional<torch::
   p.cols = static_cast<int>(x.size(1));
   p.tile_cols = static_cast<int>(cb);
   p.vec = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && (p.ld * x.element_size()) % 16 == 0;
-  if (q.has_value()) {
-    p.q = static_cast<uint8_t*>(q->data_ptr());
-    p.s = s->data_ptr<uint8_t>();
-  }
-  if (qt.has_value()) {
-    p.qt = static_cast<uint8_t*>(qt->data_ptr());
-    p.st = st->data_ptr<uint8_t>();
-  }
-  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  p.q = q.data;
+  p.s = q.scale;
+  p.qt = t.data;
+  p.st = t.scale;
+  const bool e5m2 = q.data != nullptr ? q.e5m2 : t.e5m2;
   const int ctas = static_cast<int>(rb * cb);
-  if (x.scalar_type() == at::kBFloat16) quantize<__nv_bfloat16>(p, e5m2, tile, ctas, stream);
-  else if (x.scalar_type() == at::kFloat) quantize<float>(p, e5m2, tile, ctas, stream);
-  else TORCH_CHECK(false, "quantize_fp8: bf16 or fp32 input");
+  if (x.scalar_type() == at::kBFloat16) quantize<__nv_bfloat16>(p, e5m2, tile, ctas, early, stream);
+  else quantize<float>(p, e5m2, tile, ctas, early, stream);
 }
 
-// c (+)= a b^T of quantised matrices: a [M, K'], b [N, K'] codes with their scale atoms.
-void gemm_fp8(const torch::Tensor& a, const torch::Tensor& sa, const torch::Tensor& b, const torch::Tensor& sb,
-              torch::Tensor& c, bool accumulate, int64_t status_ptr) {
+void check_input(const torch::Tensor& x, const char* what) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.size(0) > 0 && x.size(1) > 0 && (x.stride(1) == 1 || x.size(1) == 1), what,
+              ": CUDA matrix with unit column stride");
+  TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kFloat, what, ": bf16 or fp32 input");
+}
+
+// c (+)= a b^T; c checked against a and b here.
+void gemm_into(const Matrix& a, const Matrix& b, torch::Tensor& c, bool accumulate, int64_t status_ptr,
+               cudaStream_t stream) {
   using namespace mvp::fp8gemm;
-  const bool a5 = is_e5m2(a, "gemm_fp8"), b5 = is_e5m2(b, "gemm_fp8");
-  TORCH_CHECK(a.is_cuda() && a.dim() == 2 && b.dim() == 2 && a.is_contiguous() && b.is_contiguous() &&
-                  a.size(1) == b.size(1) && a.size(1) % BK == 0 && a.size(0) > 0 && b.size(0) > 0 && a.size(1) > 0,
-              "gemm_fp8: contiguous codes with the same whole blocks of 128");
-  TORCH_CHECK(a.size(0) < (int64_t(1) << 31) - 512 && b.size(0) < (int64_t(1) << 31) - 512 &&
-                  a.size(1) < (int64_t(1) << 31) - 512,
+  TORCH_CHECK(a.cols == b.cols, "gemm_fp8: reduction sizes differ");
+  constexpr int64_t kMost = (int64_t(1) << 31) - 512;
+  const int64_t kb = blocks_of(a.cols), groups = (kb + 3) / 4, ra = blocks_of(a.rows), rb = blocks_of(b.rows);
+  TORCH_CHECK(a.rows < kMost && b.rows < kMost && kb * BLOCK < kMost && (ra + 2) * groups < kMost &&
+                  (rb + 2) * groups < kMost && ((ra + 1) / 2) * rb < kMost,
               "gemm_fp8: sizes");
-  const int64_t kb = a.size(1) / BK, groups = (kb + 3) / 4;
-  const int64_t ra = (a.size(0) + HALF - 1) / HALF, rb = (b.size(0) + HALF - 1) / HALF;
-  TORCH_CHECK((ra + 2) * groups < (int64_t(1) << 31) && (rb + 2) * groups < (int64_t(1) << 31) &&
-                  ((ra + 1) / 2) * ((rb + 1) / 2) < (int64_t(1) << 31) - 1024,
-              "gemm_fp8: sizes");
-  auto scales = [&](const torch::Tensor& s, int64_t blocks) {
-    TORCH_CHECK(s.device() == a.device() && s.scalar_type() == at::kByte && s.is_contiguous() &&
-                    s.numel() == blocks * groups * ATOM,
-                "gemm_fp8: scale bytes");
-  };
-  scales(sa, ra);
-  scales(sb, rb);
-  TORCH_CHECK(b.device() == a.device() && c.device() == a.device() && c.dim() == 2 && c.size(0) == a.size(0) &&
-                  c.size(1) == b.size(0) && (c.stride(1) == 1 || c.size(1) == 1) &&
+  TORCH_CHECK(c.dim() == 2 && c.size(0) == a.rows && c.size(1) == b.rows && (c.stride(1) == 1 || c.size(1) == 1) &&
                   (c.size(0) == 1 || c.stride(0) >= c.size(1)),
-              "gemm_fp8: output [M, N] with unit column stride on the operands' device");
+              "gemm_fp8: output [M, N] with unit column stride");
   TORCH_CHECK(c.scalar_type() == at::kFloat || (c.scalar_type() == at::kBFloat16 && !accumulate),
               "gemm_fp8: bf16 or fp32 output, fp32 to accumulate");
-  for (const torch::Tensor* t : {&a, &b, &sa, &sb})
-    TORCH_CHECK((reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0, "gemm_fp8: 16-byte aligned operands");
-  const at::cuda::CUDAGuard guard(a.device());
+  const int sms = mvp::num_sms(c.get_device());
+  const int tn = choose_tile(a.rows, b.rows, static_cast<int>(kb), sms);
   CUtensorMap t[4];
   const auto u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
-  encode(&t[0], u8, a.data_ptr(), a.size(1), a.size(0), a.size(1), BK, HALF, CU_TENSOR_MAP_SWIZZLE_128B);
-  encode(&t[1], u8, b.data_ptr(), b.size(1), b.size(0), b.size(1), BK, HALF, CU_TENSOR_MAP_SWIZZLE_128B);
+  encode(&t[0], u8, a.data, kb * BLOCK, a.rows, kb * BLOCK, BK, HALF, CU_TENSOR_MAP_SWIZZLE_128B);
+  encode(&t[1], u8, b.data, kb * BLOCK, b.rows, kb * BLOCK, BK, tn / 2, CU_TENSOR_MAP_SWIZZLE_128B);
   const auto u32 = CU_TENSOR_MAP_DATA_TYPE_UINT32;
-  encode(&t[2], u32, sa.data_ptr(), ATOM / 4, ra * groups, ATOM, ATOM / 4, 1, CU_TENSOR_MAP_SWIZZLE_NONE);
-  encode(&t[3], u32, sb.data_ptr(), ATOM / 4, rb * groups, ATOM, ATOM / 4, 1, CU_TENSOR_MAP_SWIZZLE_NONE);
+  encode(&t[2], u32, a.scale, ATOM / 4, ra * groups, ATOM, ATOM / 4, 1, CU_TENSOR_MAP_SWIZZLE_NONE);
+  encode(&t[3], u32, b.scale, ATOM / 4, rb * groups, ATOM, ATOM / 4, 1, CU_TENSOR_MAP_SWIZZLE_NONE);
   Params p{};
-  p.M = static_cast<int>(a.size(0));
-  p.N = static_cast<int>(b.size(0));
+  p.M = static_cast<int>(a.rows);
+  p.N = static_cast<int>(b.rows);
   p.num_kb = static_cast<int>(kb);
   p.sf_groups = static_cast<int>(groups);
   p.C = c.data_ptr();
   p.ldc = c.stride(0);
-  p.idesc = make_idesc(a5, b5);
+  p.idesc = make_idesc(a.e5m2, b.e5m2, tn);
+  p.vec = (reinterpret_cast<uintptr_t>(p.C) & 15) == 0 && (p.ldc * c.element_size()) % 16 == 0;
   p.status = reinterpret_cast<int*>(status_ptr);
-  const int sms = mvp::num_sms(a.get_device());
+  const int epi = c.scalar_type() == at::kBFloat16 ? kStoreBf16 : accumulate ? kAccumF32 : kStoreF32;
+  if (tn == 256) launch_tile<256>(epi, t, p, sms, stream);
+  else if (tn == 192) launch_tile<192>(epi, t, p, sms, stream);
+  else launch_tile<128>(epi, t, p, sms, stream);
+}
+
+}  // namespace
+
+// {codes, scales} of x's rows and {codes, scales} of its columns (undefined where not asked for); tile: 128 x 128 blocks
+// instead of 1 x 128.
+std::vector<torch::Tensor> quantize_fp8(const torch::Tensor& x, bool tile, bool rows, bool columns, bool e5m2) {
+  check_input(x, "quantize_fp8");
+  TORCH_CHECK(rows || columns, "quantize_fp8: nothing to write");
+  const at::cuda::CUDAGuard guard(x.device());
+  std::vector<torch::Tensor> out(4);
+  Matrix q, t;
+  if (rows) q = new_matrix(x.size(0), x.size(1), e5m2, x, out[0], out[1]);
+  if (columns) t = new_matrix(x.size(1), x.size(0), e5m2, x, out[2], out[3]);
+  quantize_into(x, tile, q, t, false, at::cuda::getCurrentCUDAStream());
+  return out;
+}
+
+// c (+)= a b^T of quantised matrices with `cols` values per row.
+void gemm_fp8(const torch::Tensor& a, const torch::Tensor& sa, const torch::Tensor& b, const torch::Tensor& sb,
+              int64_t cols, torch::Tensor& c, bool accumulate, int64_t status_ptr) {
+  TORCH_CHECK(a.is_cuda() && c.device() == a.device(), "gemm_fp8: CUDA operands and output on one device");
+  const Matrix ma = as_matrix(a, sa, cols, a.device(), "gemm_fp8"), mb = as_matrix(b, sb, cols, a.device(), "gemm_fp8");
+  const at::cuda::CUDAGuard guard(a.device());
+  gemm_into(ma, mb, c, accumulate, status_ptr, at::cuda::getCurrentCUDAStream());
+}
+
+// Forward of ops.linear_fp8: {y, x^T codes, scales, w^T codes, scales} (the last four where asked for).  w8 / sw8: w's codes
+// kept by the caller.
+std::vector<torch::Tensor> linear_fp8_fwd(const torch::Tensor& x, const torch::Tensor& w,
+                                          const c10::optional<torch::Tensor>& w8, const c10::optional<torch::Tensor>& sw8,
+                                          bool need_xt, bool need_wt, int64_t status_ptr) {
+  check_input(x, "linear_fp8");
+  check_input(w, "linear_fp8");
+  TORCH_CHECK(x.device() == w.device() && x.size(1) == w.size(1), "linear_fp8: x [T, K] and w [N, K] on one device");
+  const at::cuda::CUDAGuard guard(x.device());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  if (c.scalar_type() == at::kBFloat16) launch<kStoreBf16>(t, p, sms, stream);
-  else if (!accumulate) launch<kStoreF32>(t, p, sms, stream);
-  else launch<kAccumF32>(t, p, sms, stream);
+  const int64_t T = x.size(0), K = x.size(1), N = w.size(0);
+  const bool own_w = !w8.has_value();
+  int64_t bytes = 0;
+  Matrix mx, mw, mxt, mwt;
+  place(mx, T, K, false, nullptr, bytes);
+  if (own_w) place(mw, N, K, false, nullptr, bytes);
+  auto buf = torch::empty({bytes}, x.options().dtype(at::kByte));
+  bytes = 0;
+  place(mx, T, K, false, buf.data_ptr<uint8_t>(), bytes);
+  if (own_w) place(mw, N, K, false, buf.data_ptr<uint8_t>(), bytes);
+  else {
+    TORCH_CHECK(sw8.has_value(), "linear_fp8: scales of the kept weight");
+    mw = as_matrix(*w8, *sw8, K, x.device(), "linear_fp8");
+    TORCH_CHECK(mw.rows == N, "linear_fp8: the kept weight has another shape");
+  }
+  std::vector<torch::Tensor> out(5);
+  if (need_xt) mxt = new_matrix(K, T, false, x, out[1], out[2]);
+  if (need_wt && own_w) mwt = new_matrix(K, N, false, x, out[3], out[4]);
+  out[0] = torch::empty({T, N}, x.options().dtype(at::kBFloat16));
+  quantize_into(x, false, mx, mxt, false, stream);
+  if (own_w) quantize_into(w, true, mw, mwt, true, stream);
+  gemm_into(mx, mw, out[0], false, status_ptr, stream);
+  return out;
+}
+
+// Backward of ops.linear_fp8: {dx, dw} (undefined where not asked for; dw goes into acc when that is given).
+std::vector<torch::Tensor> linear_fp8_bwd(const torch::Tensor& dy, const c10::optional<torch::Tensor>& xt,
+                                          const c10::optional<torch::Tensor>& sxt,
+                                          const c10::optional<torch::Tensor>& wt,
+                                          const c10::optional<torch::Tensor>& swt, bool e5m2,
+                                          c10::optional<torch::Tensor> acc, int64_t status_ptr) {
+  check_input(dy, "linear_fp8");
+  const at::cuda::CUDAGuard guard(dy.device());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  const int64_t T = dy.size(0), N = dy.size(1);
+  const bool need_dw = xt.has_value(), need_dx = wt.has_value();
+  TORCH_CHECK((need_dw || need_dx) && need_dw == sxt.has_value() && need_dx == swt.has_value(), "linear_fp8: operands");
+  Matrix mxt, mwt, md, mdt;
+  if (need_dw) mxt = as_matrix(*xt, *sxt, T, dy.device(), "linear_fp8");
+  if (need_dx) mwt = as_matrix(*wt, *swt, N, dy.device(), "linear_fp8");
+  int64_t bytes = 0;
+  if (need_dx) place(md, T, N, e5m2, nullptr, bytes);
+  if (need_dw) place(mdt, N, T, e5m2, nullptr, bytes);
+  auto buf = torch::empty({bytes}, dy.options().dtype(at::kByte));
+  bytes = 0;
+  if (need_dx) place(md, T, N, e5m2, buf.data_ptr<uint8_t>(), bytes);
+  if (need_dw) place(mdt, N, T, e5m2, buf.data_ptr<uint8_t>(), bytes);
+  std::vector<torch::Tensor> out(2);
+  if (need_dx) out[0] = torch::empty({T, mwt.rows}, dy.options().dtype(at::kBFloat16));
+  if (need_dw && !acc.has_value()) out[1] = torch::empty({N, mxt.rows}, dy.options().dtype(at::kBFloat16));
+  if (need_dw && acc.has_value())
+    TORCH_CHECK(acc->device() == dy.device() && acc->scalar_type() == at::kFloat,
+                "linear_fp8: fp32 accumulator on the gradient's device");
+  quantize_into(dy, false, md, mdt, false, stream);
+  if (need_dx) gemm_into(md, mwt, out[0], false, status_ptr, stream);
+  if (need_dw) gemm_into(mdt, mxt, acc.has_value() ? *acc : out[1], acc.has_value(), status_ptr, stream);
+  return out;
 }

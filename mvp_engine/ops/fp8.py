@@ -9,6 +9,7 @@ plain torch operations.
 
 from __future__ import annotations
 
+import os
 from typing import Optional
 
 import torch
@@ -23,9 +24,8 @@ _MAX_EXPONENT = {torch.float8_e4m3fn: 8, torch.float8_e5m2: 15}
 
 
 def _native(t: torch.Tensor) -> bool:
-    from . import _native as native
-
-    return native(t)
+    # as ops._native, without asking for the device that a CUDA tensor proves
+    return t.is_cuda and (os.environ.get("MVP_ALLOW_EAGER", "0") != "1" or _ext.available())
 
 
 class Fp8Matrix:
@@ -81,10 +81,6 @@ def _up(n: int, m: int) -> int:
     return -(-n // m) * m
 
 
-def _scale_shape(rows: int, blocks: int) -> tuple[int, ...]:
-    return (-(-rows // BLOCK), -(-blocks // 4), 32, 4, 4)
-
-
 def _pack_scale(byte: torch.Tensor) -> torch.Tensor:
     rows, blocks = byte.shape
     p = byte.new_zeros(_up(rows, BLOCK), _up(blocks, 4))
@@ -112,12 +108,6 @@ def _quantize_plain(x: torch.Tensor, tile: bool, dtype: torch.dtype) -> Fp8Matri
     return Fp8Matrix(q.to(dtype), _pack_scale(byte), cols)
 
 
-def _empty(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> Fp8Matrix:
-    blocks = -(-cols // BLOCK)
-    return Fp8Matrix(torch.empty(rows, blocks * BLOCK, dtype=dtype, device=device),
-                     torch.empty(_scale_shape(rows, blocks), dtype=torch.uint8, device=device), cols)
-
-
 def quantize_fp8(x: torch.Tensor, block: str = "row", *, rows: bool = True, columns: bool = False,
                  dtype: torch.dtype = torch.float8_e4m3fn) -> tuple[Optional[Fp8Matrix], Optional[Fp8Matrix]]:
     """``(matrix, transposed)`` of ``x [R, C]`` (bf16 or fp32) in 8-bit blocks, in one pass over ``x``.
@@ -137,17 +127,14 @@ def quantize_fp8(x: torch.Tensor, block: str = "row", *, rows: bool = True, colu
         raise TypeError(f"quantize_fp8: bf16 or fp32 values, got {x.dtype}")
     if not (rows or columns):
         raise ValueError("quantize_fp8: neither rows nor columns asked for")
-    x = x.detach()
     if not _native(x):
+        x = x.detach()
         return (_quantize_plain(x, block == "tile", dtype) if rows else None,
                 _quantize_plain(x.t(), block == "tile", dtype) if columns else None)
     if x.stride(1) != 1 and x.shape[1] > 1:
         x = x.contiguous()
-    q = _empty(x.shape[0], x.shape[1], dtype, x.device) if rows else None
-    t = _empty(x.shape[1], x.shape[0], dtype, x.device) if columns else None
-    _ext.ext().quantize_fp8(x, block == "tile", q.data if rows else None, q.scale if rows else None,
-                            t.data if columns else None, t.scale if columns else None)
-    return q, t
+    q, s, t, st = _ext.ext().quantize_fp8(x, block == "tile", bool(rows), bool(columns), dtype == torch.float8_e5m2)
+    return (Fp8Matrix(q, s, x.shape[1]) if rows else None, Fp8Matrix(t, st, x.shape[0]) if columns else None)
 
 
 def gemm_fp8(a: Fp8Matrix, b: Fp8Matrix, *, out: Optional[torch.Tensor] = None, accumulate: bool = False,
@@ -173,8 +160,23 @@ def gemm_fp8(a: Fp8Matrix, b: Fp8Matrix, *, out: Optional[torch.Tensor] = None, 
         res = a.dequantize() @ b.dequantize().t()
         out.add_(res) if accumulate else out.copy_(res)
         return out
-    _ext.ext().gemm_fp8(a.data, a.scale, b.data, b.scale, out, accumulate, _ext.status_buffer(a.device).data_ptr())
+    _ext.ext().gemm_fp8(a.data, a.scale, b.data, b.scale, a.cols, out, accumulate,
+                        _ext.status_buffer(a.device).data_ptr())
     return out
+
+
+def _forward(x2, w, w8, need_xt, need_wt):
+    """``(y, [x^T codes, scales, w^T codes, scales])``; what is not needed is ``None``."""
+    if _native(x2):
+        y, *kept = _ext.ext().linear_fp8_fwd(x2, w, w8[0].data if w8 else None, w8[0].scale if w8 else None,
+                                             need_xt, need_wt, _ext.status_buffer(x2.device).data_ptr())
+        if need_wt and w8:
+            kept[2:] = [w8[1].data, w8[1].scale]
+        return y, kept
+    x8, xt8 = quantize_fp8(x2, "row", rows=True, columns=need_xt)
+    q, t = w8 if w8 else quantize_fp8(w, "tile", rows=True, columns=need_wt)
+    y = gemm_fp8(x8, q, out_dtype=torch.float32).to(x2.dtype)
+    return y, [v for m, need in ((xt8, need_xt), (t, need_wt)) for v in ((m.data, m.scale) if need else (None, None))]
 
 
 class _LinearFp8(torch.autograd.Function):
@@ -182,35 +184,36 @@ class _LinearFp8(torch.autograd.Function):
     its own reduction.  What is kept for the backward is 8 bits wide: x's columns and w's."""
 
     @staticmethod
-    def forward(ctx, x2, w, w8, wt8, need_dx, need_dw, grad_dtype, acc):
-        x8, xt8 = quantize_fp8(x2, "row", rows=True, columns=need_dw)
-        if w8 is None:
-            w8, wt8 = quantize_fp8(w, "tile", rows=True, columns=need_dx)
-        y = gemm_fp8(x8, w8, out_dtype=torch.bfloat16 if x2.is_cuda else torch.float32)
-        ctx.save_for_backward(*(t for m in (xt8 if need_dw else None, wt8 if need_dx else None) if m is not None
-                                for t in (m.data, m.scale)))
+    def forward(ctx, x2, w, w8, need_dx, need_dw, grad_dtype, acc):
+        y, kept = _forward(x2, w, w8, need_dw, need_dx)
+        ctx.save_for_backward(*kept)
         ctx.meta = (need_dx, need_dw, grad_dtype, acc, x2.shape, w.shape, w.dtype, x2.dtype)
-        return y.to(x2.dtype)
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         need_dx, need_dw, grad_dtype, acc, x_shape, w_shape, w_dtype, x_dtype = ctx.meta
-        saved = list(ctx.saved_tensors)
-        if dy.stride(1) != 1:
+        xt, sxt, wt, swt = ctx.saved_tensors
+        if dy.stride(1) != 1 and dy.shape[1] > 1:
             dy = dy.contiguous()
-        dy8, dyt8 = quantize_fp8(dy, "row", rows=need_dx, columns=need_dw, dtype=grad_dtype)
+        if _native(dy):
+            dx, dw = _ext.ext().linear_fp8_bwd(dy, xt if need_dw else None, sxt if need_dw else None,
+                                               wt if need_dx else None, swt if need_dx else None,
+                                               grad_dtype == torch.float8_e5m2, acc,
+                                               _ext.status_buffer(dy.device).data_ptr())
+            return dx, dw, None, None, None, None, None
         dx = dw = None
+        dy8, dyt8 = quantize_fp8(dy.float(), "row", rows=need_dx, columns=need_dw, dtype=grad_dtype)
         if need_dw:
-            xt8 = Fp8Matrix(saved.pop(0), saved.pop(0), x_shape[0])
+            xt8 = Fp8Matrix(xt, sxt, x_shape[0])
             if acc is not None:
                 gemm_fp8(dyt8, xt8, out=acc, accumulate=True)
             else:
-                dw = gemm_fp8(dyt8, xt8, out_dtype=w_dtype if dy.is_cuda else torch.float32).to(w_dtype)
+                dw = gemm_fp8(dyt8, xt8, out_dtype=torch.float32).to(w_dtype)
         if need_dx:
-            wt8 = Fp8Matrix(saved.pop(0), saved.pop(0), w_shape[0])
-            dx = gemm_fp8(dy8, wt8, out_dtype=torch.bfloat16 if dy.is_cuda else torch.float32).to(x_dtype)
-        return dx, dw, None, None, None, None, None, None
+            dx = gemm_fp8(dy8, Fp8Matrix(wt, swt, w_shape[0]), out_dtype=torch.float32).to(x_dtype)
+        return dx, dw, None, None, None, None, None
 
 
 def linear_fp8(x: torch.Tensor, w: torch.Tensor, w8: Optional[tuple[Fp8Matrix, Fp8Matrix]] = None, *,
@@ -231,7 +234,7 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor, w8: Optional[tuple[Fp8Matrix, F
         raise ValueError(f"linear_fp8: x on {x.device}, w on {w.device}")
     if grad_dtype not in _MAX_EXPONENT:
         raise TypeError(f"linear_fp8: grad_dtype must be float8_e4m3fn or float8_e5m2, got {grad_dtype}")
-    if _native(x):
+    if x.is_cuda and _native(x):
         if x.dtype != torch.bfloat16:
             x = x.to(torch.bfloat16)
         if w.dtype != torch.bfloat16:
@@ -249,9 +252,12 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor, w8: Optional[tuple[Fp8Matrix, F
         raise ValueError("linear_fp8: the gradient accumulator must be fp32 of the weight's shape")
     need_dx = grad and x.requires_grad
     need_dw = grad and (w.requires_grad or (acc is not None and need_dx))
-    x2 = x.reshape(-1, x.shape[-1])
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if x2.stride(1) != 1 and x2.shape[1] > 1:
         x2 = x2.contiguous()
-    q, t = w8 if w8 is not None else (None, None)
-    y = _LinearFp8.apply(x2, w, q, t, need_dx, need_dw, grad_dtype, acc if need_dw else None)
-    return y.view(*x.shape[:-1], w.shape[0])
+    if need_dx or need_dw:
+        y = _LinearFp8.apply(x2, w, w8, need_dx, need_dw, grad_dtype, acc if need_dw else None)
+    else:
+        with torch.no_grad():
+            y = _forward(x2, w, w8, False, False)[0]
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0])
