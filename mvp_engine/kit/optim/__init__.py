@@ -2,8 +2,9 @@
 
 ``build_optimizer(model, "AdamW", lr, wd)`` returns the fused flat-shard AdamW
 when ``model`` is the native data-parallel runtime (same update rule as
-``torch.optim.AdamW``), and ``getattr(torch.optim, name)`` over the trainable
-parameters otherwise.
+``torch.optim.AdamW``), ``"Muon"`` there the fused Muon with AdamW for what is not
+a hidden matrix, and ``getattr(torch.optim, name)`` over the trainable parameters
+otherwise.
 """
 
 from __future__ import annotations
@@ -25,6 +26,10 @@ class OptimKit:
                 from ...parallel.optim import FlatAdamW
 
                 return FlatAdamW(base, lr=lr, weight_decay=weight_decay, **kwargs)
+            if optimizer == "Muon":
+                from ...parallel.optim import FlatMuon
+
+                return FlatMuon(base, lr=lr, weight_decay=weight_decay, **kwargs)
             assert hasattr(torch.optim, optimizer), f"Optimizer '{optimizer}' not found in torch.optim."
             opt = getattr(torch.optim, optimizer)(list(base.shard_params), lr=lr, weight_decay=weight_decay, **kwargs)
             return base.attach_optimizer(opt)

@@ -178,6 +178,10 @@ class Qwen3DecoderLayer(nn.Module):
         tp = getattr(self, "_tp", None)  # tensor-parallel runtime (column / row-parallel shards)
         Hq, Hkv, D = attn.num_heads, attn.num_kv_heads, attn.head_dim
         cp = ctx.cp
+        if ctx.fp8_linear:
+            if tp is not None or cp is not None:
+                raise ValueError("8-bit linear layers do not combine with tensor or context parallelism")
+            return self._forward_fp8(x, residual, ctx)
         if tp is None and (cp is None or not cp.ulysses_fused(x, Hq, Hkv, D)):
             return self._forward_plain(x, residual, ctx)
         if residual is None:
@@ -242,6 +246,30 @@ class Qwen3DecoderLayer(nn.Module):
         return ops.swiglu_linear(gu, _as_compute(self.mlp.down_proj.weight, gu)), h2
 
 
+    def _forward_fp8(self, x: torch.Tensor, residual: Optional[torch.Tensor], ctx: "PackedContext"):
+        """The layer with its four products in 8-bit blocks (``ops.linear_fp8``); norms, attention and the
+        residual stream as in the other paths."""
+        attn = self.self_attn
+        Hq, Hkv, D = attn.num_heads, attn.num_kv_heads, attn.head_dim
+        if residual is None:
+            hn, h = self.input_layernorm(x), x
+        else:
+            hn, h = self.input_layernorm(x, residual)
+        qkv = ops.linear_fp8(hn, self.fused_weight("qkv", hn))
+        wq, wk = _as_compute(attn.q_norm.weight, hn), _as_compute(attn.k_norm.weight, hn)
+        if ctx.causal:
+            o = ops.qk_norm_rope_attention(qkv, Hq, Hkv, wq, wk, ctx.position_ids, ctx.rope,
+                                           attn.q_norm.variance_epsilon, ctx.cu_seqlens, ctx.max_seqlen,
+                                           attn.scaling)
+        else:
+            q, k = ops.qk_norm_rope(qkv, Hq, Hkv, wq, wk, ctx.position_ids, ctx.rope, attn.q_norm.variance_epsilon)
+            o = ctx.attention(q, k, qkv[:, (Hq + Hkv) * D:].view(-1, Hkv, D), attn.scaling)
+        o = ops.linear_fp8(o.reshape(o.shape[0], Hq * D), _as_compute(attn.o_proj.weight, hn))
+        hn2, h2 = self.post_attention_layernorm(o, h)
+        gu = ops.linear_fp8(hn2, self.fused_weight("gate_up", hn2))
+        return ops.linear_fp8(ops.swiglu(gu), _as_compute(self.mlp.down_proj.weight, gu)), h2
+
+
 @dataclass
 class PackedContext:
     """Per-micro-batch metadata shared by every layer."""
@@ -252,6 +280,7 @@ class PackedContext:
     rope: ops.RopeCache
     cp: Any = None  # context-parallel runtime (ring / ulysses), or None
     causal: bool = True
+    fp8_linear: bool = False  # the decoder layers' products in 8-bit blocks
 
     def attention(self, q, k, v, scale):
         if self.cp is not None:
@@ -269,6 +298,7 @@ class Qwen3Model(nn.Module):
         self.rope = ops.RopeCache(config.head_dim, config.rope_theta, max_positions=config.max_position_embeddings)
         self.gradient_checkpointing = False
         self.checkpoint_layers: Optional[int] = None  # None: all layers when enabled
+        self.fp8_linear = False  # see Qwen3ForCausalLM.set_linear_precision
 
     def embed(self, input_ids: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
         w = _as_compute(self.embed_tokens.weight, torch.empty(0, dtype=dtype))
@@ -348,6 +378,13 @@ class Qwen3ForCausalLM(nn.Module):
     def gradient_checkpointing_disable(self) -> None:
         self.model.gradient_checkpointing = False
 
+    def set_linear_precision(self, precision: str) -> None:
+        """``"fp8"``: the decoder layers' projections run in 8-bit blocks of 128 (``ops.linear_fp8``), forward and
+        backward; ``"bf16"`` (the default): as 16-bit products.  Embedding, attention, norms and the LM head stay."""
+        if precision not in ("bf16", "fp8"):
+            raise ValueError(f"linear precision must be 'bf16' or 'fp8', got {precision!r}")
+        self.model.fp8_linear = precision == "fp8"
+
     # ------------------------------------------------------------------ init
     @torch.no_grad()
     def init_param_(self, fqn: str, t: torch.Tensor, seed: Optional[int] = None) -> None:
@@ -389,7 +426,7 @@ class Qwen3ForCausalLM(nn.Module):
         pos = position_ids.reshape(-1, T) if position_ids.dim() <= 2 else position_ids.reshape(position_ids.shape[0], -1)
         if input_ids.is_cuda:  # RoPE tables cover every position of the longest document
             self.model.rope.tables(input_ids.device, int(max_length_q))
-        return PackedContext(pos, cu, int(max_length_q), self.model.rope, cp=cp)
+        return PackedContext(pos, cu, int(max_length_q), self.model.rope, cp=cp, fp8_linear=self.model.fp8_linear)
 
     def forward(self, input_ids: torch.Tensor, *args: Any, **kwargs: Any) -> dict:
         """The model manages its own precision (bf16 operands, fp32 accumulation and statistics);

@@ -27,7 +27,7 @@ import torch.nn.functional as F
 
 from . import _ext
 from .fp8 import Fp8Matrix, gemm_fp8, linear_fp8, quantize_fp8
-from .muon import muon_lr_ratio, muon_step_, orthogonalize
+from .muon import NS_COEFFICIENTS, NS_EPS, NS_STEPS, muon_lr_ratio, muon_step_, orthogonalize
 
 __all__ = [
     "gemm",

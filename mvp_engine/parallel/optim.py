@@ -14,7 +14,7 @@ schedulers (e.g. transformers' cosine schedule) drive it unchanged.
 
 from __future__ import annotations
 
-from typing import Any, Optional
+from typing import Any, Callable, Optional, Sequence
 
 import torch
 
@@ -90,3 +90,145 @@ class FlatAdamW(torch.optim.Optimizer):
             for k in ("lr", "betas", "eps", "weight_decay", "initial_lr"):
                 if k in groups[0]:
                     self.param_groups[0][k] = groups[0][k]
+
+
+def is_hidden_matrix(fqn: str, shape: Sequence[int]) -> bool:
+    """The parameters :class:`FlatMuon` orthogonalises by default: matrices other than embeddings and output heads."""
+    return len(shape) == 2 and not any(k in fqn for k in ("embed", "lm_head", "head.weight"))
+
+
+class FlatMuon(FlatAdamW):
+    """Muon over the native data-parallel runtime: hidden matrices take orthogonalised momentum updates
+    (``ops.muon_step_``), everything else (embeddings, the head, norms, biases) the fused AdamW update.
+
+    ``lr``, ``weight_decay``, ``momentum``, ``nesterov``, ``ns_coefficients``, ``eps``, ``ns_steps`` and
+    ``adjust_lr_fn`` are those of ``torch.optim.Muon``, except that ``adjust_lr_fn`` defaults to
+    ``"match_rms_adamw"``, since one learning rate drives both kinds; ``adamw_lr_ratio`` scales it for the AdamW part,
+    whose other settings are ``betas`` and ``adamw_eps``.  ``matrix_filter(fqn, shape)`` decides which matrices are
+    orthogonalised (default :func:`is_hidden_matrix`).
+
+    On one rank the matrices of one shape go through the kernels together, momentum, products and the new bf16 weights
+    in one chain.  Across ranks a matrix lies in several shards: each rank updates its momentum, the unit's
+    updates are gathered, and a rank orthogonalises the matrices that its shard holds a part of.  The momentum lives in
+    the first AdamW moment (``exp_avg`` in checkpoints); the second stays zero for matrices.  Matrices split over a
+    tensor-parallel group are not supported.
+    """
+
+    def __init__(self, fsdp: NativeFSDP, lr: float = 1e-3, weight_decay: float = 0.1, momentum: float = 0.95,
+                 nesterov: bool = True, ns_coefficients: Sequence[float] = ops.NS_COEFFICIENTS, eps: float = ops.NS_EPS,
+                 ns_steps: int = ops.NS_STEPS, adjust_lr_fn: Optional[str] = "match_rms_adamw",
+                 betas: tuple[float, float] = (0.9, 0.95), adamw_eps: float = 1e-8, adamw_lr_ratio: float = 1.0,
+                 matrix_filter: Optional[Callable[[str, Sequence[int]], bool]] = None, **unused: Any) -> None:
+        if fsdp.tp_world > 1:
+            raise ValueError("FlatMuon: matrices split over a tensor-parallel group are not supported")
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError(f"FlatMuon: momentum must be in [0, 1), got {momentum}")
+        ops.muon_lr_ratio(1, 1, adjust_lr_fn)  # refuses unknown names
+        super().__init__(fsdp, lr=lr, betas=betas, eps=adamw_eps, weight_decay=weight_decay)
+        self.param_groups[0].update(momentum=momentum, nesterov=nesterov, ns_eps=eps)
+        self._ns = dict(steps=int(ns_steps), coefficients=tuple(float(c) for c in ns_coefficients))
+        self._adjust = adjust_lr_fn
+        self._adamw_lr_ratio = float(adamw_lr_ratio)
+        keep = matrix_filter if matrix_filter is not None else is_hidden_matrix
+        self._matrices = {id(u): [e for e in u.entries if len(e.shape) == 2 and e.numel and keep(e.fqns[0], tuple(e.shape))]
+                          for u in self.units}
+
+    def _rest(self, u: Any) -> list[tuple[int, int]]:
+        """The ranges of a unit's flat buffer that AdamW updates: what lies between the matrices."""
+        out, at = [], 0
+        for e in sorted(self._matrices[id(u)], key=lambda e: e.offset):
+            if e.offset > at:
+                out.append((at, e.offset))
+            at = e.offset + e.numel
+        if at < u.padded:
+            out.append((at, u.padded))
+        return out
+
+    @torch.no_grad()
+    def step(self, closure: Optional[Any] = None):
+        loss = closure() if closure is not None else None
+        f = self.fsdp
+        f.finish_grad_sync()
+        self._step_count += 1
+        g = self.param_groups[0]
+        b1, b2 = g["betas"]
+        lr, wd = float(g["lr"]), float(g["weight_decay"])
+        clip = dict(grad_scale=f._grad_scale, norm_sq=f._norm_sq,
+                    max_norm=f._max_norm if f._max_norm is not None else 0.0)
+        stacks: dict[tuple[int, ...], list[tuple]] = {}
+        for u in self.units:
+            lo, hi = u.local_range(f.rank)
+            own = u.own_compute_slice(f.rank)
+            master, grad = u.master.data, u.grad_shard[: u.shard]
+            shadow = own if own.dtype == torch.bfloat16 else None
+            for a, b in self._rest(u):
+                a, b = max(a, lo) - lo, min(b, hi) - lo
+                if a < b:
+                    ops.adamw_step_(master[a:b], grad[a:b], u.exp_avg[a:b], u.exp_avg_sq[a:b],
+                                    lr=lr * self._adamw_lr_ratio, beta1=b1, beta2=b2, eps=float(g["eps"]),
+                                    weight_decay=wd, step=self._step_count,
+                                    p_bf16=shadow[a:b] if shadow is not None else None, **clip)
+            if f.world == 1:
+                for e in self._matrices[id(u)]:
+                    at = slice(e.offset, e.offset + e.numel)
+                    stacks.setdefault(tuple(e.shape), []).append(
+                        tuple(t[at].view(e.shape) for t in (master, grad, u.exp_avg) + ((own,) if shadow is not None else ())))
+            else:
+                self._sharded_step(u, master, grad, lr, wd, clip)
+        for same in stacks.values():
+            cols = list(zip(*same))
+            ops.muon_step_(cols[0], cols[1], cols[2], lr=lr, momentum=float(g["momentum"]), nesterov=bool(g["nesterov"]),
+                           weight_decay=wd, eps=float(g["ns_eps"]), adjust_lr=self._adjust,
+                           p_bf16=cols[3] if len(cols) > 3 else None, **self._ns, **clip)
+        for u in self.units:
+            own = u.own_compute_slice(f.rank)
+            lo, _ = u.local_range(f.rank)
+            if own.dtype != torch.bfloat16:
+                own.copy_(u.master.to(own.dtype))
+            elif f.world > 1:  # the matrices' part; AdamW has written its own
+                for e in self._matrices[id(u)]:
+                    a, b = max(e.offset - lo, 0), min(e.offset + e.numel - lo, u.shard)
+                    if a < b:
+                        own[a:b].copy_(u.master.data[a:b])
+        f.after_optimizer_step()
+        return loss
+
+    def _sharded_step(self, u: Any, master: torch.Tensor, grad: torch.Tensor, lr: float, wd: float,
+                      clip: dict[str, Any]) -> None:
+        """Muon on a unit whose matrices lie across the shards of the data-parallel group."""
+        if not self._matrices[id(u)]:
+            return
+        f, g = self.fsdp, self.param_groups[0]
+        mu = float(g["momentum"])
+        scale: Any = clip["grad_scale"]
+        if clip["norm_sq"] is not None:  # on the device: no synchronisation
+            scale = scale * (clip["max_norm"] / (clip["norm_sq"].sqrt() * scale + 1e-6)).clamp(max=1.0)
+        lo, _ = u.local_range(f.rank)
+        update = torch.zeros(u.shard, dtype=torch.float32, device=master.device)
+        for e in self._matrices[id(u)]:
+            a, b = max(e.offset - lo, 0), min(e.offset + e.numel - lo, u.shard)
+            if a < b:
+                ga, m = grad[a:b] * scale, u.exp_avg[a:b]
+                m.lerp_(ga, 1 - mu)
+                update[a:b] = ga.lerp(m, mu) if g["nesterov"] else m
+        full = f._full_fp32(u, update)
+        for e in self._matrices[id(u)]:
+            a, b = max(e.offset - lo, 0), min(e.offset + e.numel - lo, u.shard)
+            if a >= b:
+                continue
+            o = ops.orthogonalize(full[e.offset:e.offset + e.numel].view(e.shape), eps=float(g["ns_eps"]),
+                                  out_dtype=torch.float32, **self._ns)
+            part = o.view(-1)[lo + a - e.offset:lo + b - e.offset]
+            master[a:b].mul_(1.0 - lr * wd).add_(part, alpha=-lr * ops.muon_lr_ratio(*e.shape, self._adjust))
+
+    def load_checkpoint_state_dict(self, sd: dict[str, Any], full: bool = False) -> None:
+        super().load_checkpoint_state_dict(sd, full)
+        groups = sd.get("param_groups") or []
+        if groups:
+            for k in ("momentum", "nesterov", "ns_eps"):
+                if k in groups[0]:
+                    self.param_groups[0][k] = groups[0][k]
+
+    def _group_meta(self, fqns: list[str]) -> dict[str, Any]:
+        g = self.param_groups[0]
+        return {**super()._group_meta(fqns), "momentum": g["momentum"], "nesterov": g["nesterov"], "ns_eps": g["ns_eps"]}

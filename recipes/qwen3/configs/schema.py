@@ -2,8 +2,9 @@
 
 Same fields and batching rules as the reference; additions: ``data.dataset_source``
 (e.g. ``synthetic_text``), ``model.gradient_checkpointing.num_layers`` (recompute
-only the first N layers) and ``model.config_overrides`` (architecture fields
-on top of the preset / config.json).
+only the first N layers), ``model.linear_precision`` (``fp8``: decoder projections in
+8-bit blocks) and ``model.config_overrides`` (architecture fields on top of the
+preset / config.json).
 """
 
 from __future__ import annotations
@@ -72,6 +73,7 @@ class Qwen3ModelConfig(BaseModel):
     gradient_checkpointing: Qwen3GradientCheckpointingConfig = Field(default_factory=Qwen3GradientCheckpointingConfig)
     freeze_llm: bool = False
     compile: Qwen3CompileConfig = Field(default_factory=Qwen3CompileConfig)
+    linear_precision: Literal["bf16", "fp8"] = "bf16"
     config_overrides: dict[str, Any] = Field(default_factory=dict)
 
     @field_validator("pretrained_model_name_or_path", mode="before")

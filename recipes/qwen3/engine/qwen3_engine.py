@@ -110,6 +110,8 @@ class Qwen3Engine(Engine):
         logger.info(f"Model name: {type(model).__name__}")
         model = self.model_kit.apply_model_patches(model, [patch_qwen3_model_flops])
         model = self.token_loss_kit.apply_chunked_token_loss_patch(model)
+        if m.linear_precision != "bf16":
+            model.set_linear_precision(m.linear_precision)
         model = self.model_kit.apply_freeze_policy(model, freeze_llm=m.freeze_llm)
         if build_device != "meta":
             for p in model.parameters():
