@@ -26,7 +26,7 @@
 // Work.  A and A A are symmetric: only tiles on and below the diagonal are computed, and the epilogue writes a
 // tile and its mirror, which makes an iteration s^2 l + s^3 + 2 s^2 l operations instead of 4 s^2 l + 2 s^3.
 // One launch per product handles a whole stack of same-shaped matrices.  The kernel is the pair-of-SMs GEMM
-// (256 x 256 tile per cluster, see gemm2sm_sm100.cu for the roles) over 3-D tensor maps.
+// (256 x 256 or 256 x 128 tile per cluster, see gemm2sm_sm100.cu for the roles) over 3-D tensor maps.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -46,20 +46,21 @@ namespace muon {
 using namespace gemm2;
 
 constexpr int BK = 64;
-constexpr int TILE = 256;
+constexpr int TM = 256;                  // tiles are 256 x TN, TN = 256 or 128 (choose_tile)
 constexpr int HALF = 128;
 constexpr int STAGES = 5;
-constexpr int OP_BYTES = HALF * BK * 2;  // 16 KB of A and 16 KB of B per stage and CTA
-constexpr int STAGE_BYTES = 2 * OP_BYTES;
+constexpr int A_BYTES = HALF * BK * 2;   // per stage and CTA; of B half a tile's columns
+template <int TN>
+constexpr int kStageBytes = A_BYTES + TN / 2 * BK * 2;
 constexpr int CHUNK = 32;                 // columns the epilogue handles at a time
-constexpr int CHUNKS = 128 / CHUNK;       // per warp and tile
 constexpr int HALF_BUF = 32 * CHUNK * 2;  // a warp's 32 rows of a chunk in fp16
 constexpr int EPI_BUF = 2 * HALF_BUF;     // hi and lo, or fp32
 constexpr int EPI_BYTES = 8 * 2 * EPI_BUF;  // two buffers for each warp
 constexpr int TMEM_COLS = 512;
 constexpr int EPI_WARPS = 8;             // two for each quarter of the accumulator's lanes, half of the columns each
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + 1024 + 256;
+template <int TN>
+constexpr int kSmemBytes = STAGES * kStageBytes<TN> + EPI_BYTES + 1024 + 256;
 constexpr int kMaxStack = 64;  // matrices per launch (their pointers travel as kernel parameters)
 
 // What the epilogue does with the fp32 accumulator `acc` of a tile.
@@ -116,16 +117,19 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 __device__ __forceinline__ void cp_async_wait_but_one() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
-// Tile t of a matrix: the lower triangle row by row for symmetric products, else 8-row groups.
-template <bool SYM>
+// Tile t of a matrix: symmetric products take the 256-row blocks on and below the diagonal, row by row (the block on the
+// diagonal whole, so that only blocks below it are mirrored), others 8-row groups.
+template <bool SYM, int TN>
 __device__ __forceinline__ void tile_of(const Params& p, int t, int& tm, int& tn) {
   if constexpr (SYM) {
-    tm = static_cast<int>((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
-    while (tm * (tm + 1) / 2 > t) --tm;
-    while ((tm + 1) * (tm + 2) / 2 <= t) ++tm;
-    tn = t - tm * (tm + 1) / 2;
+    constexpr int R = TM / TN;  // tiles per block
+    const int block = t / R;
+    tm = static_cast<int>((sqrtf(8.f * block + 1.f) - 1.f) * 0.5f);
+    while (tm * (tm + 1) / 2 > block) --tm;
+    while ((tm + 1) * (tm + 2) / 2 <= block) ++tm;
+    tn = (block - tm * (tm + 1) / 2) * R + t % R;
   } else {
-    const int num_m = (p.M + TILE - 1) / TILE, num_n = (p.N + TILE - 1) / TILE;
+    const int num_m = (p.M + TM - 1) / TM, num_n = (p.N + TN - 1) / TN;
     constexpr int kGroup = 8;
     const int per_group = kGroup * num_n;
     const int g = t / per_group, first = g * kGroup;
@@ -151,16 +155,18 @@ __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-template <bool A_MN, bool B_MN, int EPI, typename OUT>
+template <bool A_MN, bool B_MN, int EPI, typename OUT, int TN>
 __global__ void __launch_bounds__(THREADS, 1)
     ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p,
                       const __grid_constant__ Outs outs) {
   constexpr bool SYM = EPI == kGram || EPI == kPoly;
+  constexpr int B_BYTES = kStageBytes<TN> - A_BYTES;
+  constexpr int CHUNKS = TN / 2 / CHUNK;  // per epilogue warp and tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
-  uint8_t* sB = smem + STAGES * OP_BYTES;
-  uint8_t* sE = smem + STAGES * STAGE_BYTES;
+  uint8_t* sB = smem + STAGES * A_BYTES;
+  uint8_t* sE = smem + STAGES * kStageBytes<TN>;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(sE + EPI_BYTES);               // used in the leader
   uint64_t* empty_bar = full_bar + STAGES;                                        // both CTAs
   uint64_t* tfull_bar = empty_bar + STAGES;                                       // [2] both CTAs
@@ -215,18 +221,18 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int t = cluster_id; ok && t < total; t += clusters) {
         const int b = t / p.tiles;
         int tm, tn;
-        tile_of<SYM>(p, t - b * p.tiles, tm, tn);
-        const int m0 = tm * TILE + crank * HALF, n0 = tn * TILE + crank * HALF;
+        tile_of<SYM, TN>(p, t - b * p.tiles, tm, tn);
+        const int m0 = tm * TM + crank * HALF, n0 = tn * TN + crank * (TN / 2);
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1, abort_flag, p.status, kTimeoutProducer)) {
             ok = false;
             break;
           }
-          if (crank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * STAGE_BYTES);
+          if (crank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * kStageBytes<TN>);
           issued = true;
           const uint32_t bar = leader_full0 + stage * 8;
-          uint8_t* a_dst = sA + stage * OP_BYTES;
-          uint8_t* b_dst = sB + stage * OP_BYTES;
+          uint8_t* a_dst = sA + stage * A_BYTES;
+          uint8_t* b_dst = sB + stage * B_BYTES;
           const int k0 = kb * BK;
           if constexpr (!A_MN) {
             tma_load_3d_pair(a_dst, &tmA, bar, k0, m0, b);
@@ -238,7 +244,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             tma_load_3d_pair(b_dst, &tmB, bar, k0, n0, b);
           } else {
             tma_load_3d_pair(b_dst, &tmB, bar, n0, k0, b);
-            tma_load_3d_pair(b_dst + 64 * BK * 2, &tmB, bar, n0 + 64, k0, b);
+            if constexpr (TN == 256) tma_load_3d_pair(b_dst + 64 * BK * 2, &tmB, bar, n0 + 64, k0, b);
           }
           if (++stage == STAGES) {
             stage = 0;
@@ -256,7 +262,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   } else if (warp == 1) {
     // ----------------------------------------------------------------- MMA (leader only)
     if (crank == 0 && elect_one_sync()) {
-      constexpr uint32_t idesc = make_idesc_f16(TILE, TILE, A_MN, B_MN);
+      constexpr uint32_t idesc = make_idesc_f16(TM, TN, A_MN, B_MN);
       int stage = 0;
       uint32_t phase = 0;
       int local = 0;
@@ -266,15 +272,15 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t acc_phase = (local >> 1) & 1;
         if (!mbar_wait_bounded(&tempty_bar[acc], acc_phase ^ 1, abort_flag, p.status, kTimeoutMma)) break;
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * TILE;
+        const uint32_t d_tmem = tmem_base + acc * TN;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait_bounded(&full_bar[stage], phase, abort_flag, p.status, kTimeoutMma)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a_base = smem_u32(sA + stage * OP_BYTES);
-          const uint32_t b_base = smem_u32(sB + stage * OP_BYTES);
+          const uint32_t a_base = smem_u32(sA + stage * A_BYTES);
+          const uint32_t b_base = smem_u32(sB + stage * B_BYTES);
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k) {
             uint64_t adesc, bdesc;
@@ -306,7 +312,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint8_t* const bufs = sE + ew * 2 * EPI_BUF;
     const uint32_t leader_tempty0 = mapa_shared(smem_u32(&tempty_bar[0]), 0);
     const int row_in_tile = static_cast<int>(crank) * HALF + sub * 32;
-    const int col_in_tile = (ew / 4) * 128;
+    const int col_in_tile = (ew / 4) * (TN / 2);
     // byte offset of 16-byte piece j of row r: 64-byte rows (fp16) and 128-byte rows (fp32), both free of conflicts for
     // lanes that read or write the same piece of 8 rows
     auto piece16 = [](int r, int j) { return r * 64 + ((j ^ ((r >> 1) & 3)) << 4); };
@@ -317,13 +323,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (t < total) {
           const int b = t / p.tiles;
           int tm, tn;
-          tile_of<SYM>(p, t - b * p.tiles, tm, tn);
-          const int n = tn * TILE + col_in_tile + (seq % CHUNKS) * CHUNK + (lane & 3) * 8;
+          tile_of<SYM, TN>(p, t - b * p.tiles, tm, tn);
+          const int n = tn * TN + col_in_tile + (seq % CHUNKS) * CHUNK + (lane & 3) * 8;
           const int64_t mat = static_cast<int64_t>(b) * p.M * p.ld;
           const uint32_t dst = smem_u32(bufs + (seq & 1) * EPI_BUF);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int r = i * 8 + lane / 4, m = tm * TILE + row_in_tile + r;
+            const int r = i * 8 + lane / 4, m = tm * TM + row_in_tile + r;
             const bool ok = m < p.M && n < p.ld;  // the columns between N and ld are never used
             const int64_t at = ok ? mat + static_cast<int64_t>(m) * p.ld + n : 0;
             const uint32_t d = dst + piece16(r, lane & 3);
@@ -340,9 +346,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int t = cluster_id; t < total; t += clusters, ++local) {
       const int b = t / p.tiles;
       int tm, tn;
-      tile_of<SYM>(p, t - b * p.tiles, tm, tn);
+      tile_of<SYM, TN>(p, t - b * p.tiles, tm, tn);
       const int acc = local & 1;
-      const int m_warp = tm * TILE + row_in_tile;  // the warp's first row
+      const int m_warp = tm * TM + row_in_tile;  // the warp's first row
       const int m = m_warp + lane;
       const bool row_ok = m < p.M;
       const int64_t mat = static_cast<int64_t>(b) * p.M * p.ld;
@@ -364,13 +370,13 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll 1
       for (int c = 0; c < CHUNKS; ++c) {
         const int seq = local * CHUNKS + c;
-        const int n = tn * TILE + col_in_tile + c * CHUNK;
+        const int n = tn * TN + col_in_tile + c * CHUNK;
         uint8_t* const buf = bufs + (seq & 1) * EPI_BUF;
         const bool live = n < p.N && m_warp < p.M;  // same for all lanes
         float x[CHUNK];
         if (live) {
           uint32_t r[CHUNK];
-          tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(sub * 32) << 16) + acc * TILE + col_in_tile + c * CHUNK,
+          tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(sub * 32) << 16) + acc * TN + col_in_tile + c * CHUNK,
                              r);
           if constexpr (EPI != kGram) {
             float by_col = 0.f;  // lane j: what column n + j adds to beta
@@ -452,7 +458,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               }
             }
             if constexpr (SYM) {
-              if (tm != tn && row_ok) {  // mirror: a warp's 32 rows are 64 contiguous bytes of each mirrored row
+              if (tn * TN + TN <= tm * TM && row_ok) {  // mirror: a warp's 32 rows are 64 contiguous bytes of each mirrored row
                 __half* d = p.D_hi + mat + static_cast<int64_t>(n) * p.ld + m;
 #pragma unroll
                 for (int j = 0; j < CHUNK; ++j)
@@ -757,29 +763,59 @@ __global__ void __launch_bounds__(kStartThreads) ns_first_kernel(const __grid_co
 }
 
 // ------------------------------------------------------------------------- host side
-// Tensor map of a stack [count, rows, cols] of fp16 matrices with row stride ld.
-inline void make_map(CUtensorMap* map, const __half* base, int cols, int rows, int count, int ld, bool mn_major) {
+// A product's operand: a stack [count, rows, cols] of fp16 matrices with row stride ld.
+struct Operand {
+  const __half* base;
+  int cols, rows, ld;
+};
+
+// Its tensor map; mn_major: boxes of 64 columns x BK rows, else of 64 columns (the reduction) x box_rows rows.
+inline void make_map(CUtensorMap* map, const Operand& o, int count, bool mn_major, int box_rows) {
   ensure_thread_context();
-  cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(count)};
-  cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * 2, static_cast<cuuint64_t>(ld) * 2 * rows};
-  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(mn_major ? BK : HALF), 1};
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(o.cols), static_cast<cuuint64_t>(o.rows), static_cast<cuuint64_t>(count)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(o.ld) * 2, static_cast<cuuint64_t>(o.ld) * 2 * o.rows};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(mn_major ? BK : box_rows), 1};
   cuuint32_t es[3] = {1, 1, 1};
-  const CUresult r = encode_tiled_fn()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(base), dims,
+  const CUresult r = encode_tiled_fn()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(o.base), dims,
                                        strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   TORCH_CHECK(r == CUDA_SUCCESS, "orthogonalize: cuTensorMapEncodeTiled failed with code ", static_cast<int>(r));
 }
 
-template <bool A_MN, bool B_MN, int EPI, typename OUT = float>
-void product(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, const Outs& outs, int sms,
-             cudaStream_t stream) {
-  auto kern = ns_product_kernel<A_MN, B_MN, EPI, OUT>;
+// Tiles of one matrix.
+inline int64_t tiles_of(bool sym, int M, int N, int tn) {
+  const int64_t m = (M + TM - 1) / TM;
+  return sym ? m * (m + 1) / 2 * (TM / tn) : m * ((N + tn - 1) / tn);
+}
+
+// Tile width with the shorter schedule.  A tile's MMAs take 512 cycles per k-block at TN = 256 and about 350 at 128 (A's share
+// of the shared-memory traffic grows); its read-out, which overlaps the next tile's MMAs, about 5500 cycles (A),
+// 9500 (B) and 12500 (X) at 256 and half of that at 128 (both from time stamps of single tiles).
+inline int choose_tile(bool sym, bool reads, int M, int N, int K, int count, int sms) {
+  const int64_t clusters = std::max(1, sms / 2), kb = (K + BK - 1) / BK;
+  int64_t cost[2];
+  for (int i = 0; i < 2; ++i) {
+    const int tn = i == 0 ? 256 : 128;
+    const int64_t waves = (tiles_of(sym, M, N, tn) * count + clusters - 1) / clusters;
+    const int64_t mma = kb * (i == 0 ? 512 : 350), out = (sym ? (reads ? 9500 : 5500) : 12500) >> i;
+    cost[i] = waves * std::max(mma, out) + std::min(mma, out);
+  }
+  return cost[1] < cost[0] ? 128 : 256;
+}
+
+template <bool A_MN, bool B_MN, int EPI, typename OUT, int TN>
+void launch(const Operand& a, const Operand& b, Params p, const Outs& outs, int sms, cudaStream_t stream) {
+  CUtensorMap ta, tb;
+  make_map(&ta, a, p.count, A_MN, HALF);
+  make_map(&tb, b, p.count, B_MN, TN / 2);
+  p.tiles = static_cast<int>(tiles_of(EPI == kGram || EPI == kPoly, p.M, p.N, TN));
+  auto kern = ns_product_kernel<A_MN, B_MN, EPI, OUT, TN>;
   static std::atomic<uint64_t> configured{0};
-  allow_smem(kern, SMEM_BYTES, configured);
+  allow_smem(kern, kSmemBytes<TN>, configured);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * std::min(p.tiles * p.count, std::max(1, sms / 2)));
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.dynamicSmemBytes = kSmemBytes<TN>;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -791,6 +827,14 @@ void product(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, cons
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, p, outs));
+}
+
+template <bool A_MN, bool B_MN, int EPI, typename OUT = float>
+void product(const Operand& a, const Operand& b, const Params& p, const Outs& outs, int sms, cudaStream_t stream) {
+  if (choose_tile(EPI == kGram || EPI == kPoly, EPI != kGram, p.M, p.N, p.K, p.count, sms) == 256)
+    launch<A_MN, B_MN, EPI, OUT, 256>(a, b, p, outs, sms, stream);
+  else
+    launch<A_MN, B_MN, EPI, OUT, 128>(a, b, p, outs, sms, stream);
 }
 
 struct Shape {
@@ -834,17 +878,11 @@ struct Workspace {
 template <typename Last>
 void iterate(const Shape& s, Workspace& w, int steps, double a, double b, double c, int* status, int sms,
              cudaStream_t stream, Last last) {
-  const int tiles_s = (s.short_side + TILE - 1) / TILE;
-  const int tiles_m = (s.rows + TILE - 1) / TILE, tiles_n = (s.cols + TILE - 1) / TILE;
   const Outs none{};
-  CUtensorMap sa, sb;  // A and B as K-major operands (symmetric: rows are columns)
-  make_map(&sa, w.A, s.short_side, s.short_side, s.count, s.lds, false);
-  make_map(&sb, w.B, s.short_side, s.short_side, s.count, s.lds, false);
+  const Operand A{w.A, s.short_side, s.short_side, s.lds}, B{w.B, s.short_side, s.short_side, s.lds};
   for (int it = 0; it < steps; ++it) {
     const int cur = it & 1;
-    CUtensorMap xk, xmn;  // X as a K-major operand (rows) and as an MN-major one (columns)
-    make_map(&xk, w.hi[cur], s.cols, s.rows, s.count, s.ldx, false);
-    make_map(&xmn, w.hi[cur], s.cols, s.rows, s.count, s.ldx, true);
+    const Operand X{w.hi[cur], s.cols, s.rows, s.ldx};
     Params p{};
     p.count = s.count;
     p.status = status;
@@ -853,14 +891,13 @@ void iterate(const Shape& s, Workspace& w, int steps, double a, double b, double
     // A' = tau A = (tau / sigma^2) X' X'^T
     p.M = p.N = s.short_side;
     p.K = s.tall ? s.rows : s.cols;
-    p.tiles = tiles_s * (tiles_s + 1) / 2;
     p.ld = s.lds;
     p.alpha = s.tau / s.sigma / s.sigma;
     p.beta = 0.f;
     p.D_hi = w.A;
     p.diag = w.diag_a;
-    if (s.tall) product<true, true, kGram>(xmn, xmn, p, none, sms, stream);
-    else product<false, false, kGram>(xk, xk, p, none, sms, stream);
+    if (s.tall) product<true, true, kGram>(X, X, p, none, sms, stream);
+    else product<false, false, kGram>(X, X, p, none, sms, stream);
     // B' = tau (b A + c A A), off the diagonal (b + c (a_i + a_j)) A' + (c / tau) A' A' with A' zero on it
     p.K = s.short_side;
     p.alpha = static_cast<float>(c / s.tau);
@@ -870,12 +907,11 @@ void iterate(const Shape& s, Workspace& w, int steps, double a, double b, double
     p.gamma = static_cast<float>(c);
     p.diag_a = w.diag_a;
     p.diag = w.diag_b;
-    product<false, false, kPoly>(sa, sa, p, none, sms, stream);
+    product<false, false, kPoly>(A, A, p, none, sms, stream);
     // X' <- a X' + (1 / tau) B' X'   (or X' B')
     p.M = s.rows;
     p.N = s.cols;
     p.K = s.short_side;
-    p.tiles = tiles_m * tiles_n;
     p.ld = s.ldx;
     p.alpha = 1.f / s.tau;
     p.beta = static_cast<float>(a);
@@ -885,13 +921,13 @@ void iterate(const Shape& s, Workspace& w, int steps, double a, double b, double
     if (it + 1 < steps) {
       p.D_hi = w.hi[cur ^ 1];
       p.D_lo = w.lo;  // in place: each element is read and written by one thread
-      if (s.tall) product<false, false, kNext>(xk, sb, p, none, sms, stream);
-      else product<false, true, kNext>(sb, xmn, p, none, sms, stream);
+      if (s.tall) product<false, false, kNext>(X, B, p, none, sms, stream);
+      else product<false, true, kNext>(B, X, p, none, sms, stream);
     } else {
       p.alpha /= s.sigma;
       p.beta /= s.sigma;
       p.diag_scale /= s.sigma;
-      last(s.tall ? xk : sb, s.tall ? sb : xmn, p);
+      last(s.tall ? X : B, s.tall ? B : X, p);
     }
   }
 }
@@ -947,7 +983,7 @@ void check_sizes(int64_t rows, int64_t cols, int64_t steps, const std::vector<do
 }
 
 template <typename OUT>
-void last_out(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, const Outs& o, bool tall, int sms,
+void last_out(const Operand& ta, const Operand& tb, const Params& p, const Outs& o, bool tall, int sms,
               cudaStream_t stream) {
   if (tall) product<false, false, kOut, OUT>(ta, tb, p, o, sms, stream);
   else product<false, true, kOut, OUT>(ta, tb, p, o, sms, stream);
@@ -987,7 +1023,7 @@ void orthogonalize(const torch::Tensor& x, torch::Tensor& out, int64_t steps, co
     else TORCH_CHECK(false, "orthogonalize: fp32, bf16 or fp16 input");
     iterate(s, w, static_cast<int>(steps), coefficients[0], coefficients[1], coefficients[2],
             reinterpret_cast<int*>(status_ptr), sms, stream,
-            [&](const CUtensorMap& ta, const CUtensorMap& tb, const Params& p) {
+            [&](const Operand& ta, const Operand& tb, const Params& p) {
               if (out.scalar_type() == at::kFloat) last_out<float>(ta, tb, p, outs, s.tall, sms, stream);
               else if (out.scalar_type() == at::kBFloat16) last_out<__nv_bfloat16>(ta, tb, p, outs, s.tall, sms, stream);
               else if (out.scalar_type() == at::kHalf) last_out<__half>(ta, tb, p, outs, s.tall, sms, stream);
@@ -1050,7 +1086,7 @@ void muon_step_(const std::vector<torch::Tensor>& p, const std::vector<torch::Te
     start<float, true>(ins, q, s, ctas, stream);
     iterate(s, w, static_cast<int>(steps), coefficients[0], coefficients[1], coefficients[2],
             reinterpret_cast<int*>(status_ptr), sms, stream,
-            [&](const CUtensorMap& ta, const CUtensorMap& tb, Params l) {
+            [&](const Operand& ta, const Operand& tb, Params l) {
               l.rate = static_cast<float>(rate);
               l.decay = static_cast<float>(decay);
               if (s.tall) product<false, false, kStep>(ta, tb, l, outs, sms, stream);
