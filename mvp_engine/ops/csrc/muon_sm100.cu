@@ -790,17 +790,19 @@ inline int64_t tiles_of(bool sym, int M, int N, int tn) {
 
 // Tile width with the shorter schedule.  A tile's MMAs take 512 cycles per k-block at TN = 256 and about 350 at 128 (A's share
 // of the shared-memory traffic grows); its read-out, which overlaps the next tile's MMAs, about 5500 cycles (A),
-// 9500 (B) and 12500 (X) at 256 and half of that at 128 (both from time stamps of single tiles).
+// 9500 (B) and 12500 (X) at 256 and half of that at 128 (both from time stamps of single tiles).  Beyond two waves of the
+// narrow tiles memory sets the pace and the wide ones win (12 x 1024 x 4096: 1.16 ms wide, 1.23 ms narrow; a Muon step on
+// 3 x 1001 x 777: 267 us wide, 202 us narrow).
 inline int choose_tile(bool sym, bool reads, int M, int N, int K, int count, int sms) {
   const int64_t clusters = std::max(1, sms / 2), kb = (K + BK - 1) / BK;
-  int64_t cost[2];
+  int64_t cost[2], waves = 0;
   for (int i = 0; i < 2; ++i) {
     const int tn = i == 0 ? 256 : 128;
-    const int64_t waves = (tiles_of(sym, M, N, tn) * count + clusters - 1) / clusters;
+    waves = (tiles_of(sym, M, N, tn) * count + clusters - 1) / clusters;
     const int64_t mma = kb * (i == 0 ? 512 : 350), out = (sym ? (reads ? 9500 : 5500) : 12500) >> i;
     cost[i] = waves * std::max(mma, out) + std::min(mma, out);
   }
-  return cost[1] < cost[0] ? 128 : 256;
+  return waves <= 2 && cost[1] < cost[0] ? 128 : 256;
 }
 
 template <bool A_MN, bool B_MN, int EPI, typename OUT, int TN>
