@@ -578,7 +578,8 @@ struct StartParams {
   double* partial;     // [count, parts] sums of squares, added in index order by every reader
   __half* hi;
   __half* lo;
-  float sigma, eps;
+  float sigma;
+  double eps;
   float momentum;
   int nesterov;
   float grad_scale;
@@ -704,7 +705,7 @@ __global__ void __launch_bounds__(kStartThreads) ns_first_kernel(const __grid_co
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     const double norm = sqrt(s);
     // a norm that is not a number stays one
-    if (threadIdx.x == 0) factor_s = static_cast<double>(p.sigma) / (norm < p.eps ? static_cast<double>(p.eps) : norm);
+    if (threadIdx.x == 0) factor_s = static_cast<double>(p.sigma) / (norm < p.eps ? p.eps : norm);
   }
   __syncthreads();
   const double factor = factor_s;
@@ -941,7 +942,7 @@ inline int64_t group_size(int64_t rows, int64_t cols, int64_t count) {
   return std::min<int64_t>(count, std::min<int64_t>(kMaxStack, fit));
 }
 
-inline StartParams start_params(const Shape& s, Workspace& w, torch::Tensor& partial, float eps) {
+inline StartParams start_params(const Shape& s, Workspace& w, torch::Tensor& partial, double eps) {
   StartParams q{};
   q.rows = s.rows;
   q.cols = s.cols;
@@ -1012,7 +1013,7 @@ void orthogonalize(const torch::Tensor& x, torch::Tensor& out, int64_t steps, co
     Workspace w(s, x.device());
     const int ctas = start_ctas(s, sms);
     auto partial = torch::empty({s.count, ctas}, x.options().dtype(at::kDouble));
-    StartParams q = start_params(s, w, partial, static_cast<float>(eps));
+    StartParams q = start_params(s, w, partial, eps);
     Ins ins{};
     Outs outs{};
     for (int i = 0; i < s.count; ++i) {
@@ -1071,7 +1072,7 @@ void muon_step_(const std::vector<torch::Tensor>& p, const std::vector<torch::Te
     Workspace w(s, dev);
     const int ctas = start_ctas(s, sms);
     auto partial = torch::empty({s.count, ctas}, p[0].options().dtype(at::kDouble));
-    StartParams q = start_params(s, w, partial, static_cast<float>(eps));
+    StartParams q = start_params(s, w, partial, eps);
     q.momentum = static_cast<float>(momentum);
     q.nesterov = nesterov ? 1 : 0;
     q.grad_scale = static_cast<float>(grad_scale);

@@ -255,6 +255,8 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor, w8: Optional[tuple[Fp8Matrix, F
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if x2.stride(1) != 1 and x2.shape[1] > 1:
         x2 = x2.contiguous()
+    if w.is_cuda and w.stride(1) != 1 and w.shape[1] > 1:
+        w = w.contiguous()
     if need_dx or need_dw:
         y = _LinearFp8.apply(x2, w, w8, need_dx, need_dw, grad_dtype, acc if need_dw else None)
     else:

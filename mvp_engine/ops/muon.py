@@ -6,6 +6,7 @@ the fp16 tensor-core kernels of ``csrc/muon_sm100.cu``; on CPU the same formulas
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Sequence, Union
 
@@ -20,19 +21,22 @@ NS_EPS = 1e-7
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def _check_iteration(steps: int, coefficients: Sequence[float], eps: float) -> tuple[int, list[float], float]:
+def _check_iteration(steps: int, coefficients: Sequence[float], eps: float) -> tuple[int, tuple[float, ...], float]:
     """Refuse iterations whose singular values leave the range the kernels' fp16 products are scaled for."""
-    steps = int(steps)
-    if steps < 1:
-        raise ValueError(f"orthogonalize: steps must be at least 1, got {steps}")
-    coef = [float(c) for c in coefficients]
+    return _checked(int(steps), tuple(float(c) for c in coefficients), float(eps))
+
+
+@functools.lru_cache(maxsize=64)
+def _checked(steps: int, coef: tuple[float, ...], eps: float) -> tuple[int, tuple[float, ...], float]:
+    if not 1 <= steps <= 1000:
+        raise ValueError(f"orthogonalize: steps must be in 1 .. 1000, got {steps}")
     if len(coef) != 3 or not all(math.isfinite(c) for c in coef):
-        raise ValueError(f"orthogonalize: three finite coefficients are needed, got {coefficients!r}")
-    if not (float(eps) > 0 and math.isfinite(float(eps))):
-        raise ValueError(f"orthogonalize: eps must be positive, got {eps!r}")
+        raise ValueError(f"orthogonalize: three finite coefficients are needed, got {coef!r}")
+    if not 1e-100 <= eps <= 1e30:
+        raise ValueError(f"orthogonalize: eps must be in 1e-100 .. 1e30, got {eps!r}")
     a, b, c = coef
     top = 1.0  # singular values lie in [0, top]; the Frobenius norm of the first X is at most 1
-    for _ in range(min(steps, 32)):
+    for _ in range(min(steps, 64)):
         # extrema of a s + b s^3 + c s^5 on [0, top] and of b t + c t^2 on [0, top^2]
         points = [top]
         disc = 9 * b * b - 20 * a * c
@@ -44,13 +48,13 @@ def _check_iteration(steps: int, coefficients: Sequence[float], eps: float) -> t
         if c != 0 and 0 < -b / (2 * c) < top * top:
             inner.append(-b / (2 * c))
         if max(abs(b * t + c * t * t) for t in inner) > 3.9:
-            raise ValueError(f"orthogonalize: coefficients {tuple(coef)} leave the range of the iteration")
+            raise ValueError(f"orthogonalize: coefficients {coef} leave the range of the iteration")
         top = max(abs(a * s + b * s**3 + c * s**5) for s in points) * 1.001  # the kernels' rounding
         if top > 1.9:
-            raise ValueError(f"orthogonalize: coefficients {tuple(coef)} let singular values grow to {top:.3g}; "
+            raise ValueError(f"orthogonalize: coefficients {coef} let singular values grow to {top:.3g}; "
                              "at most 1.9 is supported")
         top = max(top, 1e-6)
-    return steps, coef, float(eps)
+    return steps, coef, eps
 
 
 def _newton_schulz(u: torch.Tensor, steps: int, coefficients: Sequence[float], eps: float) -> torch.Tensor:
@@ -156,8 +160,8 @@ def muon_step_(
     if ps[0].numel() == 0:
         return
     ptrs = [t.data_ptr() for t in ps + ms + shadows]
-    if len(set(ptrs)) != len(ptrs):
-        raise ValueError("muon_step_: a weight, momentum or bf16 copy is given twice")
+    if len(set(ptrs)) != len(ptrs) or not set(ptrs).isdisjoint(t.data_ptr() for t in gs):
+        raise ValueError("muon_step_: a weight, momentum or bf16 copy is given twice, or as a gradient")
     rate = float(lr) * muon_lr_ratio(shape[0], shape[1], adjust_lr)
     decay = 1.0 - float(lr) * float(weight_decay)
     from . import _native
@@ -170,7 +174,8 @@ def muon_step_(
             return
         scale = float(grad_scale)
         if norm_sq is not None:
-            scale *= min(1.0, float(max_norm) / (float(norm_sq.sqrt()) * scale + 1e-6))
+            clip = float(max_norm) / (float(norm_sq.sqrt()) * scale + 1e-6)
+            scale *= 1.0 if clip > 1.0 else clip  # a norm that is not a number reaches the weights
         for i, w in enumerate(ps):
             gi = gs[i] * scale
             ms[i].lerp_(gi, 1 - momentum)

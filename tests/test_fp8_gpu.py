@@ -219,6 +219,26 @@ def test_linear_gradient_against_differences():
         assert abs(diff - float(grad.double().norm())) <= 2.0**-4 * abs(diff)
 
 
+def test_linear_strided_operands():
+    """Weights and inputs that are slices or transposes of larger tensors."""
+    big, wide = rand((140, 600), 1), rand((500, 301), 2, spread=0.0)
+    for x, w in ((big[3:133:2, 7:307], wide[:90].t()[:300].t()), (big.t()[5:65], wide[:140].t()[10:50]),
+                 (big[:, :301][:1], wide[::4])):
+        x = x[:, : min(x.shape[1], w.shape[1])]
+        w = w[:, : x.shape[1]]
+        got = ops.linear_fp8(x, w)
+        assert torch.equal(got, ops.linear_fp8(x.contiguous(), w.contiguous()))
+
+
+def test_linear_on_one_dimension_and_tokens_of_every_count():
+    w = rand((40, 72), 2, spread=0.0)
+    x = rand((300, 72), 1)
+    full = ops.linear_fp8(x, w)
+    assert torch.equal(ops.linear_fp8(x[5], w), full[5])
+    for t in (1, 2, 31, 127, 129, 255, 257):  # a row's blocks are its own: its result does not depend on the others
+        assert torch.equal(ops.linear_fp8(x[:t], w), full[:t])
+
+
 def test_linear_empty_and_no_grad():
     w = rand((32, 64), 2).requires_grad_()
     x = torch.empty(0, 64, dtype=torch.bfloat16, device="cuda", requires_grad=True)

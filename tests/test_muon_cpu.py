@@ -76,6 +76,12 @@ def test_muon_step_scale_clip_and_shadow():
     assert torch.equal(shadow, p.to(torch.bfloat16))
 
 
+def test_muon_step_nan_gradient_norm_reaches_the_weights():
+    p = torch.ones(4, 4)
+    ops.muon_step_(p, torch.ones(4, 4), torch.zeros(4, 4), lr=0.1, norm_sq=torch.tensor(float("nan")), max_norm=1.0)
+    assert torch.isnan(p).all()
+
+
 def test_lr_ratio():
     assert ops.muon_lr_ratio(100, 400) == 1.0 and ops.muon_lr_ratio(400, 100) == 2.0
     assert ops.muon_lr_ratio(400, 100, "match_rms_adamw") == pytest.approx(0.2 * 20)
@@ -104,6 +110,8 @@ def test_refusals():
     w = z(4, 4)
     with pytest.raises(ValueError):
         ops.muon_step_([w, w], [x, x], [z(4, 4), z(4, 4)], lr=0.1)
+    with pytest.raises(ValueError):
+        ops.muon_step_(z(4, 4), w, w, lr=0.1)  # the momentum is updated while the gradient is still read
     with pytest.raises(ValueError):
         ops.muon_step_(z(4, 4), x, z(4, 4), lr=0.1, p_bf16=z(4, 4))
     with pytest.raises(ValueError):
