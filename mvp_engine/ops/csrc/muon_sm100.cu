@@ -27,6 +27,9 @@
 // tile and its mirror, which makes an iteration s^2 l + s^3 + 2 s^2 l operations instead of 4 s^2 l + 2 s^3.
 // One launch per product handles a whole stack of same-shaped matrices.  The kernel is the pair-of-SMs GEMM
 // (256 x 256 or 256 x 128 tile per cluster, see gemm2sm_sm100.cu for the roles) over 3-D tensor maps.
+// Measured, five iterations: 4 x 4096 x 4096 in 4.3 to 4.7 ms (1.2 to 1.3 PFLOP/s; the bf16 GEMM settles at 1.4 under the
+// power limit), 12 x 1024 x 4096 in 1.1 ms, bound by what X's update moves through L2 (4 bytes read and 4 written per value
+// beside the operands), 1 x 256 x 512 in 105 us, bound by 17 dependent launches.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
