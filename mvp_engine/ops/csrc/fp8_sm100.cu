@@ -669,14 +669,14 @@ __global__ void __launch_bounds__(THREADS, 1)
           tmem_ld_32x32b_x32(base + c * CHUNK + CHUNK, r1);
           tmem_wait_ld();
           tc_fence_before();
-          remote_arrive(leader_handed + acc * 8);
+          remote_arrive_relaxed(leader_handed + acc * 8);
           store_chunk<EPI>(p, buf, m0, n0 + c * CHUNK, r0);
           store_chunk<EPI>(p, buf, m0, n0 + c * CHUNK + CHUNK, r1);
           first = acc == 0 ? 0 : 2;
           count = P::CHUNKS - 2;
         } else {
           tc_fence_before();
-          remote_arrive(leader_handed + acc * 8);  // this warp's part of the tile before has been read
+          remote_arrive_relaxed(leader_handed + acc * 8);  // this warp's part of the tile before has been read
         }
       }
 #pragma unroll 1
@@ -687,7 +687,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tmem_wait_ld();
         if (!P::SHARED_COLS && i == count - 1) {
           tc_fence_before();
-          remote_arrive(leader_handed + acc * 8);
+          remote_arrive_relaxed(leader_handed + acc * 8);
         }
         store_chunk<EPI>(p, buf, m0, n0 + c * CHUNK, r);
       }

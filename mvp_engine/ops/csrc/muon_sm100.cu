@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         if (c == CHUNKS - 1) {  // the accumulator has been read
           tc_fence_before();
-          remote_arrive(leader_tempty0 + acc * 8);
+          remote_arrive_relaxed(leader_tempty0 + acc * 8);
         }
         if (live) {
           if constexpr (SYM) {

@@ -24,6 +24,11 @@ __device__ __forceinline__ void cluster_sync_all() {
 __device__ __forceinline__ void remote_arrive(uint32_t cluster_bar_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar_addr) : "memory");
 }
+// The same without waiting for this thread's earlier memory writes: enough where the arrival hands back tensor memory
+// (ordered by tcgen05.wait::ld and the before_thread_sync fence) and an epilogue's stores are still under way.
+__device__ __forceinline__ void remote_arrive_relaxed(uint32_t cluster_bar_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar_addr) : "memory");
+}
 // 2-D tiled load into this CTA's shared memory whose completion is reported to the
 // barrier at cluster address `bar` (the leader CTA's).  No multicast.
 __device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const void* tmap, uint32_t bar, int c0, int c1) {
