@@ -20,6 +20,9 @@
 // only what is off them is rounded to fp16: with A = D + A~, A A = A~ A~ + (D_i + D_j) A~ + D^2 element by element, and
 // B's diagonal joins the linear term, (a + B_ii) (hi + lo).  That halves the error of well conditioned matrices
 // (simulated against 64 bits at 512 x 2048: 1.7e-3 -> 0.5e-3) and bounds it for tiny ones.
+// For small matrices, whose errors average less, a result that keeps more than 16 bits (the fp32 step or output) takes X's low
+// part into its products as well: (hi + lo)(hi + lo)^T without lo lo^T, and B (hi + lo), as two more passes and one more
+// over the reduction (Shape::split).
 // Entries then stay below 1.9 sigma and 3.9 tau (the caller checks the coefficients for it), within 65504, and
 // what underflows is 2^-24 of an average entry.
 //
@@ -95,6 +98,8 @@ struct Params {
   const float* diag_a;  // kPoly: A's diagonal
   float gamma, tau;
   float decay, rate;
+  int passes;           // over the reduction; in pass i an operand is the low part of X where bit i of its mask is set
+  uint32_t low_a, low_b;
   int* status;
 };
 
@@ -160,8 +165,9 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { retu
 
 template <bool A_MN, bool B_MN, int EPI, typename OUT, int TN>
 __global__ void __launch_bounds__(THREADS, 1)
-    ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p,
-                      const __grid_constant__ Outs outs) {
+    ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                      const __grid_constant__ CUtensorMap tmA_low, const __grid_constant__ CUtensorMap tmB_low,
+                      const Params p, const __grid_constant__ Outs outs) {
   constexpr bool SYM = EPI == kGram || EPI == kPoly;
   constexpr int B_BYTES = kStageBytes<TN> - A_BYTES;
   constexpr int CHUNKS = TN / 2 / CHUNK;  // per epilogue warp and tile
@@ -226,7 +232,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         int tm, tn;
         tile_of<SYM, TN>(p, t - b * p.tiles, tm, tn);
         const int m0 = tm * TM + crank * HALF, n0 = tn * TN + crank * (TN / 2);
-        for (int kb = 0; kb < num_kb; ++kb) {
+        for (int i = 0; i < num_kb * p.passes; ++i) {
+          const int pass = i / num_kb, kb = i - pass * num_kb;
+          const CUtensorMap* ta = (p.low_a >> pass) & 1u ? &tmA_low : &tmA;
+          const CUtensorMap* tb = (p.low_b >> pass) & 1u ? &tmB_low : &tmB;
           if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1, abort_flag, p.status, kTimeoutProducer)) {
             ok = false;
             break;
@@ -238,16 +247,16 @@ __global__ void __launch_bounds__(THREADS, 1)
           uint8_t* b_dst = sB + stage * B_BYTES;
           const int k0 = kb * BK;
           if constexpr (!A_MN) {
-            tma_load_3d_pair(a_dst, &tmA, bar, k0, m0, b);
+            tma_load_3d_pair(a_dst, ta, bar, k0, m0, b);
           } else {
-            tma_load_3d_pair(a_dst, &tmA, bar, m0, k0, b);
-            tma_load_3d_pair(a_dst + 64 * BK * 2, &tmA, bar, m0 + 64, k0, b);
+            tma_load_3d_pair(a_dst, ta, bar, m0, k0, b);
+            tma_load_3d_pair(a_dst + 64 * BK * 2, ta, bar, m0 + 64, k0, b);
           }
           if constexpr (!B_MN) {
-            tma_load_3d_pair(b_dst, &tmB, bar, k0, n0, b);
+            tma_load_3d_pair(b_dst, tb, bar, k0, n0, b);
           } else {
-            tma_load_3d_pair(b_dst, &tmB, bar, n0, k0, b);
-            if constexpr (TN == 256) tma_load_3d_pair(b_dst + 64 * BK * 2, &tmB, bar, n0 + 64, k0, b);
+            tma_load_3d_pair(b_dst, tb, bar, n0, k0, b);
+            if constexpr (TN == 256) tma_load_3d_pair(b_dst + 64 * BK * 2, tb, bar, n0 + 64, k0, b);
           }
           if (++stage == STAGES) {
             stage = 0;
@@ -276,7 +285,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (!mbar_wait_bounded(&tempty_bar[acc], acc_phase ^ 1, abort_flag, p.status, kTimeoutMma)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * TN;
-        for (int kb = 0; kb < num_kb; ++kb) {
+        for (int kb = 0; kb < num_kb * p.passes; ++kb) {
           if (!mbar_wait_bounded(&full_bar[stage], phase, abort_flag, p.status, kTimeoutMma)) {
             ok = false;
             break;
@@ -771,16 +780,17 @@ __global__ void __launch_bounds__(kStartThreads) ns_first_kernel(const __grid_co
 struct Operand {
   const __half* base;
   int cols, rows, ld;
+  const __half* low = nullptr;  // X's low part, where products read it
 };
 
 // Its tensor map; mn_major: boxes of 64 columns x BK rows, else of 64 columns (the reduction) x box_rows rows.
-inline void make_map(CUtensorMap* map, const Operand& o, int count, bool mn_major, int box_rows) {
+inline void make_map(CUtensorMap* map, const Operand& o, bool low, int count, bool mn_major, int box_rows) {
   ensure_thread_context();
   cuuint64_t dims[3] = {static_cast<cuuint64_t>(o.cols), static_cast<cuuint64_t>(o.rows), static_cast<cuuint64_t>(count)};
   cuuint64_t strides[2] = {static_cast<cuuint64_t>(o.ld) * 2, static_cast<cuuint64_t>(o.ld) * 2 * o.rows};
   cuuint32_t box[3] = {64, static_cast<cuuint32_t>(mn_major ? BK : box_rows), 1};
   cuuint32_t es[3] = {1, 1, 1};
-  const CUresult r = encode_tiled_fn()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(o.base), dims,
+  const CUresult r = encode_tiled_fn()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(low ? o.low : o.base), dims,
                                        strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   TORCH_CHECK(r == CUDA_SUCCESS, "orthogonalize: cuTensorMapEncodeTiled failed with code ", static_cast<int>(r));
@@ -812,8 +822,21 @@ inline int choose_tile(bool sym, bool reads, int M, int N, int K, int count, int
 template <bool A_MN, bool B_MN, int EPI, typename OUT, int TN>
 void launch(const Operand& a, const Operand& b, Params p, const Outs& outs, int sms, cudaStream_t stream) {
   CUtensorMap ta, tb;
-  make_map(&ta, a, p.count, A_MN, HALF);
-  make_map(&tb, b, p.count, B_MN, TN / 2);
+  make_map(&ta, a, false, p.count, A_MN, HALF);
+  make_map(&tb, b, false, p.count, B_MN, TN / 2);
+  CUtensorMap ta_low = ta, tb_low = tb;
+  p.passes = 1;
+  p.low_a = p.low_b = 0;
+  if (a.low != nullptr && b.low != nullptr) {  // X X^T: hi hi, hi lo, lo hi
+    p.passes = 3;
+    p.low_a = 0b100;
+    p.low_b = 0b010;
+  } else if (a.low != nullptr || b.low != nullptr) {  // B X: hi, lo
+    p.passes = 2;
+    p.low_a = p.low_b = 0b10;
+  }
+  if (a.low != nullptr) make_map(&ta_low, a, true, p.count, A_MN, HALF);
+  if (b.low != nullptr) make_map(&tb_low, b, true, p.count, B_MN, TN / 2);
   p.tiles = static_cast<int>(tiles_of(EPI == kGram || EPI == kPoly, p.M, p.N, TN));
   auto kern = ns_product_kernel<A_MN, B_MN, EPI, OUT, TN>;
   static std::atomic<uint64_t> configured{0};
@@ -832,12 +855,13 @@ void launch(const Operand& a, const Operand& b, Params p, const Outs& outs, int 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, p, outs));
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, ta_low, tb_low, p, outs));
 }
 
 template <bool A_MN, bool B_MN, int EPI, typename OUT = float>
 void product(const Operand& a, const Operand& b, const Params& p, const Outs& outs, int sms, cudaStream_t stream) {
-  if (choose_tile(EPI == kGram || EPI == kPoly, EPI != kGram, p.M, p.N, p.K, p.count, sms) == 256)
+  const int passes = a.low != nullptr && b.low != nullptr ? 3 : a.low != nullptr || b.low != nullptr ? 2 : 1;
+  if (choose_tile(EPI == kGram || EPI == kPoly, EPI != kGram, p.M, p.N, passes * p.K, p.count, sms) == 256)
     launch<A_MN, B_MN, EPI, OUT, 256>(a, b, p, outs, sms, stream);
   else
     launch<A_MN, B_MN, EPI, OUT, 128>(a, b, p, outs, sms, stream);
@@ -847,33 +871,40 @@ struct Shape {
   int rows, cols, count;
   int short_side, ldx, lds;
   bool tall;
+  bool split;  // X's low part takes part in the products
   float sigma, tau;
-  Shape(int64_t m, int64_t n, int64_t L)
+  // `fine`: the result keeps more than 16 bits.  The error falls with the long side (simulated against 64 bits: 6e-4 at 200 x 200,
+  // 4.9e-4 at 400 x 500, 4.1e-4 at 128 x 1000; with the low part 3.8e-4, 3.2e-4, 3.3e-4), while the extra passes cost least
+  // where a product is mostly start and end.
+  Shape(int64_t m, int64_t n, int64_t L, bool fine)
       : rows(static_cast<int>(m)), cols(static_cast<int>(n)), count(static_cast<int>(L)) {
     tall = m > n;
+    split = fine && std::max(m, n) <= 768;
     short_side = tall ? cols : rows;
     ldx = (cols + 7) / 8 * 8;
     lds = (short_side + 7) / 8 * 8;
     sigma = std::ldexp(1.f, static_cast<int>(std::min(15.0, std::round(0.5 * std::log2(static_cast<double>(m) * n)))));
     tau = std::ldexp(1.f, static_cast<int>(std::min(14.0, std::round(std::log2(static_cast<double>(short_side))))));
   }
-  // fp16 elements of the workspace: X hi twice (a product reads one while its epilogue writes the other), X lo, A, B
+  // fp16 elements of the workspace: X hi twice (a product reads one while its epilogue writes the other), X lo (twice too
+  // where products read it), A, B
   int64_t x_elems() const { return static_cast<int64_t>(count) * rows * ldx; }
   int64_t s_elems() const { return static_cast<int64_t>(count) * short_side * lds; }
-  int64_t elems() const { return 3 * x_elems() + 2 * s_elems(); }
+  int64_t elems() const { return (split ? 4 : 3) * x_elems() + 2 * s_elems(); }
 };
 
 struct Workspace {
   torch::Tensor buf;
-  __half *hi[2], *lo, *A, *B;
+  __half *hi[2], *lo[2], *A, *B;
   float *diag_a, *diag_b;
   Workspace(const Shape& s, const torch::Device& dev) {
     const int64_t diag_elems = 4 * static_cast<int64_t>(s.count) * s.lds;  // two vectors of fp32
     buf = torch::empty({s.elems() + diag_elems}, torch::TensorOptions().dtype(at::kHalf).device(dev));
     hi[0] = reinterpret_cast<__half*>(buf.data_ptr());
     hi[1] = hi[0] + s.x_elems();
-    lo = hi[1] + s.x_elems();
-    A = lo + s.x_elems();
+    lo[0] = hi[1] + s.x_elems();
+    lo[1] = s.split ? lo[0] + s.x_elems() : lo[0];
+    A = lo[1] + s.x_elems();
     B = A + s.s_elems();
     diag_a = reinterpret_cast<float*>(B + s.s_elems());
     diag_b = diag_a + static_cast<int64_t>(s.count) * s.lds;
@@ -888,7 +919,7 @@ void iterate(const Shape& s, Workspace& w, int steps, double a, double b, double
   const Operand A{w.A, s.short_side, s.short_side, s.lds}, B{w.B, s.short_side, s.short_side, s.lds};
   for (int it = 0; it < steps; ++it) {
     const int cur = it & 1;
-    const Operand X{w.hi[cur], s.cols, s.rows, s.ldx};
+    const Operand X{w.hi[cur], s.cols, s.rows, s.ldx, s.split ? w.lo[cur] : nullptr};
     Params p{};
     p.count = s.count;
     p.status = status;
@@ -923,10 +954,10 @@ void iterate(const Shape& s, Workspace& w, int steps, double a, double b, double
     p.beta = static_cast<float>(a);
     p.diag_scale = 1.f;
     p.C_hi = w.hi[cur];
-    p.C_lo = w.lo;
+    p.C_lo = w.lo[cur];
     if (it + 1 < steps) {
       p.D_hi = w.hi[cur ^ 1];
-      p.D_lo = w.lo;  // in place: each element is read and written by one thread
+      p.D_lo = w.lo[cur ^ 1];  // in place where no product reads it: each element is read and written by one thread
       if (s.tall) product<false, false, kNext>(X, B, p, none, sms, stream);
       else product<false, true, kNext>(B, X, p, none, sms, stream);
     } else {
@@ -940,7 +971,7 @@ void iterate(const Shape& s, Workspace& w, int steps, double a, double b, double
 
 // Matrices per group: bounded by the pointer table and by 2 GiB of workspace.
 inline int64_t group_size(int64_t rows, int64_t cols, int64_t count) {
-  const Shape one(rows, cols, 1);
+  const Shape one(rows, cols, 1, true);
   const int64_t fit = std::max<int64_t>(1, (int64_t(1) << 30) / std::max<int64_t>(1, one.elems()));
   return std::min<int64_t>(count, std::min<int64_t>(kMaxStack, fit));
 }
@@ -953,7 +984,7 @@ inline StartParams start_params(const Shape& s, Workspace& w, torch::Tensor& par
   q.parts = static_cast<int>(partial.size(1));
   q.partial = partial.data_ptr<double>();
   q.hi = w.hi[0];
-  q.lo = w.lo;
+  q.lo = w.lo[0];
   q.sigma = s.sigma;
   q.eps = eps;
   q.grad_scale = 1.f;
@@ -1012,7 +1043,7 @@ void orthogonalize(const torch::Tensor& x, torch::Tensor& out, int64_t steps, co
   const int64_t size = x.size(1) * x.size(2);
   const int64_t group = group_size(x.size(1), x.size(2), x.size(0));
   for (int64_t first = 0; first < x.size(0); first += group) {
-    const Shape s(x.size(1), x.size(2), std::min<int64_t>(group, x.size(0) - first));
+    const Shape s(x.size(1), x.size(2), std::min<int64_t>(group, x.size(0) - first), out.scalar_type() == at::kFloat);
     Workspace w(s, x.device());
     const int ctas = start_ctas(s, sms);
     auto partial = torch::empty({s.count, ctas}, x.options().dtype(at::kDouble));
@@ -1071,7 +1102,7 @@ void muon_step_(const std::vector<torch::Tensor>& p, const std::vector<torch::Te
   const int sms = mvp::num_sms(dev.index());
   const int64_t group = group_size(sizes[0], sizes[1], static_cast<int64_t>(count));
   for (int64_t first = 0; first < static_cast<int64_t>(count); first += group) {
-    const Shape s(sizes[0], sizes[1], std::min<int64_t>(group, static_cast<int64_t>(count) - first));
+    const Shape s(sizes[0], sizes[1], std::min<int64_t>(group, static_cast<int64_t>(count) - first), true);
     Workspace w(s, dev);
     const int ctas = start_ctas(s, sms);
     auto partial = torch::empty({s.count, ctas}, p[0].options().dtype(at::kDouble));
