@@ -48,13 +48,13 @@ struct QuantParams {
 };
 
 // Scale byte of a block from the bits of its largest magnitude: 127 + e, or -1 if it is not finite.
-// amax = 1.m 2^(E-127); MAX = 1.75 2^p, so e = E - 127 - p, one more if 1.m > 1.75.
+// amax = 1.m 2^(E-127); MAX = 1.75 2^p, so e = E - 127 - p, one more if 1.m > 1.75: adding a quarter less one unit to the
+// fraction carries into the exponent exactly then.
 template <bool E5M2>
 __device__ __forceinline__ int scale_byte(uint32_t amax_bits) {
-  const int E = static_cast<int>(amax_bits >> 23);
-  if (E == 255) return -1;
   constexpr int p = E5M2 ? 15 : 8;
-  return max(0, E - p + ((amax_bits & 0x7FFFFFu) > 0x600000u ? 1 : 0));
+  const int b = max(0, static_cast<int>((amax_bits + 0x1FFFFFu) >> 23) - p);
+  return amax_bits >= 0x7F800000u ? -1 : b;
 }
 // 2^-e for scale byte b (b <= 247, so the exponent field stays in 7..254).
 __device__ __forceinline__ float inverse_scale(int b) { return __uint_as_float(static_cast<uint32_t>(254 - b) << 23); }
@@ -63,6 +63,13 @@ __device__ __forceinline__ float inverse_scale(int b) { return __uint_as_float(s
 __device__ __forceinline__ uint2 nan_codes(int n) {
   return make_uint2(n >= 4 ? 0x7F7F7F7Fu : n <= 0 ? 0u : 0x7F7F7F7Fu >> (8 * (4 - n)),
                     n >= 8 ? 0x7F7F7F7Fu : n <= 4 ? 0u : 0x7F7F7F7Fu >> (8 * (8 - n)));
+}
+
+// 2^-e as a pair of bf16 (a power of two, so products with it are exact and subnormal ones end as zero codes either way).
+__device__ __forceinline__ __nv_bfloat162 bf16_pair(float lo, float hi) { return __floats2bfloat162_rn(lo, hi); }
+__device__ __forceinline__ uint32_t scaled2(uint32_t two, __nv_bfloat162 f) {
+  const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&two), f);
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 // Two codes, `lo` in the low byte.
@@ -125,6 +132,7 @@ __global__ void __launch_bounds__(QT, sizeof(T) == 2 ? 4 : 2) quantize_kernel(co
   __shared__ uint32_t col_max[QT / 32][BLOCK];
   __shared__ __align__(16) float col_inv[BLOCK];  // 2^-e of each column's block; 0: it is not finite
   __shared__ uint8_t col_byte[BLOCK];
+  __shared__ __align__(8) uint8_t row_byte[BLOCK];
   const int tile_r = blockIdx.x / p.tile_cols, tile_c = blockIdx.x - tile_r * p.tile_cols;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int l = threadIdx.x % 16, g = threadIdx.x / 16;
@@ -243,38 +251,69 @@ __global__ void __launch_bounds__(QT, sizeof(T) == 2 ? 4 : 2) quantize_kernel(co
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float f = inverse_scale(max(row_b[i], 0));
-      uint2 out;
       uint32_t w[4];
+      if constexpr (BF16) {
+        const __nv_bfloat162 ff = bf16_pair(f, f);
+        const uint32_t u[4] = {scaled2(v[i].u.x, ff), scaled2(v[i].u.y, ff), scaled2(v[i].u.z, ff), scaled2(v[i].u.w, ff)};
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        w[j] = codes2<E5M2>(__uint_as_float(v[i].bits(2 * j)) * f, __uint_as_float(v[i].bits(2 * j + 1)) * f);
-      out = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+        for (int j = 0; j < 4; ++j) w[j] = codes2<E5M2>(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xFFFF0000u));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          w[j] = codes2<E5M2>(__uint_as_float(v[i].bits(2 * j)) * f, __uint_as_float(v[i].bits(2 * j + 1)) * f);
+      }
+      uint2 out = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
       if (row_b[i] < 0) out = nan_codes(p.cols - c0);
       if (r0 + i < p.rows) *reinterpret_cast<uint2*>(p.q + (r0 + i) * ldq + c0) = out;
-      if (l == 0) {
-        const int rr = g * 8 + i;
-        uint8_t* a = atom + (rr % 32) * 16 + (rr / 32) * 4;
-        a[tile_c % 4] = r0 + i < p.rows ? static_cast<uint8_t>(row_b[i] < 0 ? 127 : row_b[i]) : 0;
-        if (tile_c == p.tile_cols - 1)  // blocks the atom has beyond the matrix
-          for (int b = tile_c % 4 + 1; b < 4; ++b) a[b] = 0;
-      }
+    }
+    // the scale bytes of the tile's rows, one row per thread, from the lanes that hold them
+    if (l == 0) {
+      uint32_t w[2] = {0u, 0u};
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        w[i / 4] |= static_cast<uint32_t>(r0 + i < p.rows ? (row_b[i] < 0 ? 127 : row_b[i]) : 0) << (8 * (i & 3));
+      *reinterpret_cast<uint2*>(&row_byte[g * 8]) = make_uint2(w[0], w[1]);
+    }
+    __syncthreads();
+    if (threadIdx.x < BLOCK) {
+      uint8_t* a = atom + (threadIdx.x % 32) * 16 + (threadIdx.x / 32) * 4;
+      a[tile_c % 4] = row_byte[threadIdx.x];
+      if (tile_c == p.tile_cols - 1)  // blocks the atom has beyond the matrix
+        for (int b = tile_c % 4 + 1; b < 4; ++b) a[b] = 0;
     }
   }
   if (p.qt != nullptr) {
     const int groups = (row_blocks + 3) / 4;
     const float4 inv0 = *reinterpret_cast<const float4*>(col_inv + l * 8);
     const float4 inv1 = *reinterpret_cast<const float4*>(col_inv + l * 8 + 4);
+    const float inv[8] = {inv0.x, inv0.y, inv0.z, inv0.w, inv1.x, inv1.y, inv1.z, inv1.w};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float f = j == 0 ? inv0.x : j == 1 ? inv0.y : j == 2 ? inv0.z : j == 3 ? inv0.w
-                    : j == 4 ? inv1.x : j == 5 ? inv1.y : j == 6 ? inv1.z : inv1.w;
-      uint32_t w[4];
+    for (int k = 0; k < 4; ++k) {  // columns 8 l + 2 k and the next
+      uint32_t w[2][4];
+      if constexpr (BF16) {
+        const __nv_bfloat162 ff = bf16_pair(inv[2 * k], inv[2 * k + 1]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = codes2<E5M2>(__uint_as_float(v[2 * i].bits(j)) * f, __uint_as_float(v[2 * i + 1].bits(j)) * f);
-      uint2 out = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
-      if (f == 0.f) out = nan_codes(p.rows - r0);
-      *reinterpret_cast<uint2*>(turned + (l * 8 + j) * BLOCK + (g ^ l) * 8) = out;
+        for (int i = 0; i < 4; ++i) {
+          const uint4 e = v[2 * i].u, o = v[2 * i + 1].u;
+          const uint32_t u0 = scaled2(k == 0 ? e.x : k == 1 ? e.y : k == 2 ? e.z : e.w, ff);
+          const uint32_t u1 = scaled2(k == 0 ? o.x : k == 1 ? o.y : k == 2 ? o.z : o.w, ff);
+          w[0][i] = codes2<E5M2>(__uint_as_float(u0 << 16), __uint_as_float(u1 << 16));
+          w[1][i] = codes2<E5M2>(__uint_as_float(u0 & 0xFFFF0000u), __uint_as_float(u1 & 0xFFFF0000u));
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w[h][i] = codes2<E5M2>(__uint_as_float(v[2 * i].bits(2 * k + h)) * inv[2 * k + h],
+                                   __uint_as_float(v[2 * i + 1].bits(2 * k + h)) * inv[2 * k + h]);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint2 out = make_uint2(w[h][0] | (w[h][1] << 16), w[h][2] | (w[h][3] << 16));
+        if (inv[2 * k + h] == 0.f) out = nan_codes(p.rows - r0);
+        *reinterpret_cast<uint2*>(turned + (l * 8 + 2 * k + h) * BLOCK + (g ^ l) * 8) = out;
+      }
     }
     if (threadIdx.x < BLOCK) {
       const int col = tile_c * BLOCK + threadIdx.x;
