@@ -5,6 +5,8 @@ Usage::
     python -m mvp_engine.ops.microbench gemm            # Qwen3-8B layer shapes, ours vs cuBLAS
     python -m mvp_engine.ops.microbench gemm --shape 8192,24576,4096 --iters 20
     python -m mvp_engine.ops.microbench vision          # Qwen3-VL ViT LayerNorm / bias+GELU / RoPE
+    python -m mvp_engine.ops.microbench fp8             # 8-bit quantisation and products, beside the bf16 GEMM
+    python -m mvp_engine.ops.microbench muon            # Newton-Schulz stacks of Qwen3-8B matrices
     torchrun --nproc-per-node 2 -m mvp_engine.ops.microbench cp_attention --tokens 131072
 
 Prints one JSON line per case with the kernel time and achieved TFLOP/s.
@@ -621,6 +623,41 @@ def bench_vision(tokens: int, iters: int) -> None:
         print(json.dumps(row), flush=True)
 
 
+def bench_fp8(shapes: dict[str, tuple[int, int, int]], iters: int) -> None:
+    """Quantisation and the 8-bit product per layer shape; the bf16 GEMM of the same shape as the comparison."""
+    from mvp_engine import ops
+
+    for name, (M, N, K) in shapes.items():
+        x = torch.randn(M, K, device="cuda").bfloat16()
+        w = torch.randn(N, K, device="cuda").bfloat16()
+        q, w8 = ops.quantize_fp8(x)[0], ops.quantize_fp8(w, "tile")[0]
+        acc = torch.zeros(M, N, device="cuda")
+        row = {"kernel": "fp8", "shape": name, "MNK": [M, N, K]}
+        ms = _time(lambda: ops.gemm_fp8(q, w8), iters)
+        row["product_ms"], row["product_tflops"] = round(ms, 4), round(2e-9 * M * N * K / ms, 1)
+        row["product_acc_ms"] = round(_time(lambda: ops.gemm_fp8(q, w8, out=acc, accumulate=True), iters), 4)
+        ms = _time(lambda: ops.quantize_fp8(x, columns=True), iters)
+        row["quantize_x_ms"], row["quantize_x_gbs"] = round(ms, 4), round(4e-6 * M * K / ms, 1)
+        ms = _time(lambda: ops.quantize_fp8(w, "tile", columns=True), iters)
+        row["quantize_w_ms"], row["quantize_w_gbs"] = round(ms, 4), round(4e-6 * N * K / ms, 1)
+        if _WITH_REF:
+            row["bf16_gemm_ms"] = round(_time(lambda: ops.gemm(x, w), iters), 4)
+        print(json.dumps(row))
+
+
+def bench_muon(iters: int) -> None:
+    """``ops.orthogonalize`` on stacks of Qwen3-8B matrices; FLOPs counted with symmetric products by halves."""
+    from mvp_engine import ops
+
+    for count, m, n in ((8, 1024, 4096), (4, 4096, 4096), (2, 12288, 4096), (1, 4096, 12288), (1, 256, 512)):
+        x = torch.randn(count, m, n, device="cuda")
+        s, l = min(m, n), max(m, n)
+        flops = 5.0 * count * (3.0 * s * s * l + float(s) ** 3)
+        ms = _time(lambda: ops.orthogonalize(x), iters)
+        print(json.dumps({"kernel": "orthogonalize", "stack": [count, m, n], "ms": round(ms, 4),
+                          "tflops": round(flops / ms * 1e-9, 1)}))
+
+
 def _ext_mod():
     from mvp_engine.ops import _ext
 
@@ -642,7 +679,7 @@ def _hbm_peak() -> float:
 def main() -> None:
     ap = argparse.ArgumentParser()
     ap.add_argument("what", choices=["gemm", "attention", "peer_rs", "tp_gemm", "cp_attention", "cp_layer", "vision",
-                                     "fsdp_gather", "comm_loopback"])
+                                     "fsdp_gather", "comm_loopback", "fp8", "muon"])
     ap.add_argument("--copy-ctas", type=int, default=24, help="fsdp_gather: copy CTAs carried by the GEMM")
     ap.add_argument("--loopback-world", type=int, default=2, help="fsdp_gather: local 'ranks' when run alone")
     ap.add_argument("--impls", default="ring,ring_fused,ulysses", help="cp_attention: cases to time")
@@ -657,12 +694,14 @@ def main() -> None:
     args = ap.parse_args()
     global _WITH_REF
     _WITH_REF = not args.no_ref
-    if args.what == "gemm":
+    if args.what in ("gemm", "fp8"):
         shapes = QWEN3_8B_SHAPES
         if args.shape:
             M, N, K = (int(v) for v in args.shape.split(","))
             shapes = {"custom": (M, N, K)}
-        bench_gemm(shapes, args.iters)
+        (bench_gemm if args.what == "gemm" else bench_fp8)(shapes, args.iters)
+    elif args.what == "muon":
+        bench_muon(args.iters)
     elif args.what == "tp_gemm":
         bench_tp_gemm(args.tokens if args.tokens != 8192 else 4096, args.hidden, args.iters)
     elif args.what == "peer_rs":
