@@ -224,7 +224,8 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor, w8: Optional[tuple[Fp8Matrix, F
     blocks for ``dx`` and in column blocks, with x's, for ``dw`` (``grad_dtype``: the gradient's 8-bit type).  The
     weight gradient goes into ``w._mvp_grad_acc`` when present, as in :func:`linear`.  ``w8`` is ``quantize_fp8(w, "tile",
     rows=True, columns=True)`` of the present weights, for a caller that keeps it between calls; without it the
-    call quantises ``w`` itself.  Not differentiable twice.
+    call quantises ``w`` itself.  Not differentiable twice.  A backward pass may be captured into a CUDA graph; as with every
+    torch operator, no eager autograd graph of the same leaf tensors may be alive meanwhile.
     """
     from . import grad_acc, linear
 

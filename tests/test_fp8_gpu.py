@@ -268,6 +268,56 @@ def test_linear_other_stream_and_graph():
         assert torch.equal(out, ops.linear_fp8(x, w))
 
 
+def test_calls_on_two_streams_at_once():
+    """Layers and updates under way together: each call has its own workspace, results are those of calls alone."""
+    x, w, dy = rand((700, 900), 1), rand((1100, 900), 2), rand((700, 1100), 3)
+    u = torch.randn(3, 200, 600, device="cuda", generator=torch.Generator("cuda").manual_seed(4))
+
+    def layer():
+        a, b = x.detach().requires_grad_(), w.detach().requires_grad_()
+        y = ops.linear_fp8(a, b)
+        return (y.detach(), *torch.autograd.grad(y, (a, b), dy))
+
+    want_l, want_o = layer(), ops.orthogonalize(u)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        with torch.cuda.stream(streams[0]):
+            got[0].append(layer())
+        with torch.cuda.stream(streams[1]):
+            got[1].append(ops.orthogonalize(u))
+            got[1].append(ops.linear_fp8(x, w))
+    torch.cuda.synchronize()
+    _ext.check_status()
+    for r in got[0]:
+        assert all(torch.equal(a, b) for a, b in zip(r, want_l))
+    for i, r in enumerate(got[1]):
+        assert torch.equal(r, want_o if i % 2 == 0 else want_l[0])
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 values in, codes out and products out: the far end equals the same rows by themselves."""
+    rows, cols = 65600, 33000
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    tail = rand((200, cols), 1)
+    x[:-200] = 1.0
+    x[-200:] = tail
+    q, t = ops.quantize_fp8(x, columns=True)
+    alone = ops.quantize_fp8(tail)[0]
+    assert torch.equal(q.data[-200:].view(torch.uint8), alone.data.view(torch.uint8))
+    assert torch.equal(q.exponents()[-200:], alone.exponents())
+    # the last whole column block is rows 65408 .. 65535, the rest of the matrix ends within the next
+    part = ops.quantize_fp8(x[65408:], rows=False, columns=True)[1]
+    assert torch.equal(t.data[:, 65408:].contiguous().view(torch.uint8), part.data.view(torch.uint8))
+    del x, q, t
+    a, b = rand((46400, 128), 2), rand((46400, 128), 3)
+    qa, qb = ops.quantize_fp8(a)[0], ops.quantize_fp8(b)[0]
+    y = ops.gemm_fp8(qa, qb)
+    small = ops.gemm_fp8(ops.quantize_fp8(a[-300:])[0], qb)
+    assert torch.equal(y[-300:], small)
+
+
 def test_refusals():
     x, w = rand((4, 64)), rand((8, 64))
     with pytest.raises(TypeError):
