@@ -142,8 +142,11 @@ struct AdamWArgs {
   float grad_scale;
   const float* norm_sq;  // optional: sum of squares of the unscaled grads (global)
   float max_norm;
+  bool vec;  // every array starts where four of its values can be moved at once
 };
 
+// Four values per access where the arrays are aligned for it; a slice of a flat buffer that starts elsewhere is taken one
+// value at a time.
 __global__ void adamw_kernel(AdamWArgs a) {
   float scale = a.grad_scale;
   if (a.norm_sq != nullptr) {
@@ -153,7 +156,7 @@ __global__ void adamw_kernel(AdamWArgs a) {
   }
   const float step_size = a.lr / a.bc1;
   const float decay = 1.f - a.lr * a.wd;
-  const int64_t n4 = a.n / 4;
+  const int64_t n4 = a.vec ? a.n / 4 : 0;
   for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < n4;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     float4 p = reinterpret_cast<float4*>(a.p)[i];
@@ -323,7 +326,9 @@ void adamw_step_(torch::Tensor& p, const torch::Tensor& g, torch::Tensor& m, tor
   a.norm_sq = norm_sq.has_value() ? norm_sq->data_ptr<float>() : nullptr;
   a.max_norm = static_cast<float>(max_norm);
   if (a.n == 0) return;
-  mvp::adamw_kernel<<<mvp::grid_for((a.n + 3) / 4, 256), 256, 0, at::cuda::getCurrentCUDAStream()>>>(a);
+  auto aligned = [](const void* x, uintptr_t to) { return reinterpret_cast<uintptr_t>(x) % to == 0; };
+  a.vec = aligned(a.p, 16) && aligned(a.g, 16) && aligned(a.m, 16) && aligned(a.v, 16) && aligned(a.p_bf16, 8);
+  mvp::adamw_kernel<<<mvp::grid_for(a.vec ? (a.n + 3) / 4 : a.n, 256), 256, 0, at::cuda::getCurrentCUDAStream()>>>(a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
