@@ -19,7 +19,7 @@ from typing import Any, Callable, Optional, Sequence
 import torch
 
 from .. import ops
-from .fsdp import NativeFSDP
+from .fsdp import _ALIGN, NativeFSDP
 
 
 class FlatAdamW(torch.optim.Optimizer):
@@ -134,12 +134,13 @@ class FlatMuon(FlatAdamW):
                           for u in self.units}
 
     def _rest(self, u: Any) -> list[tuple[int, int]]:
-        """The ranges of a unit's flat buffer that AdamW updates: what lies between the matrices."""
+        """The ranges of a unit's flat buffer that AdamW updates: what lies between the matrices.  A matrix ends
+        with the padding behind it (always zero), so a range starts where an entry does, aligned."""
         out, at = [], 0
         for e in sorted(self._matrices[id(u)], key=lambda e: e.offset):
             if e.offset > at:
                 out.append((at, e.offset))
-            at = e.offset + e.numel
+            at = e.offset + -(-e.numel // _ALIGN) * _ALIGN
         if at < u.padded:
             out.append((at, u.padded))
         return out
