@@ -17,6 +17,7 @@ from __future__ import annotations
 from typing import Any, Callable, Optional, Sequence
 
 import torch
+import torch.nn as nn
 
 from .. import ops
 from .fsdp import _ALIGN, NativeFSDP
@@ -93,8 +94,15 @@ class FlatAdamW(torch.optim.Optimizer):
 
 
 def is_hidden_matrix(fqn: str, shape: Sequence[int]) -> bool:
-    """The parameters :class:`FlatMuon` orthogonalises by default: matrices other than embeddings and output heads."""
-    return len(shape) == 2 and not any(k in fqn for k in ("embed", "lm_head", "head.weight"))
+    """The parameters :class:`FlatMuon` orthogonalises by default: matrices other than embeddings and output heads, which
+    are told by their names (``embed``, ``head``, ``classifier``; a head under another name needs ``matrix_filter``)."""
+    return len(shape) == 2 and not any(k in fqn for k in ("embed", "lm_head", "head.weight", "classifier"))
+
+
+def _is_hidden_entry(e: Any) -> bool:
+    """:func:`is_hidden_matrix` under every name of a parameter, none of whose owners is an embedding module."""
+    return (all(is_hidden_matrix(f, tuple(e.shape)) for f in e.fqns) and
+            not any(isinstance(mod, nn.Embedding) for mod, _ in e.owners))
 
 
 class FlatMuon(FlatAdamW):
@@ -105,7 +113,7 @@ class FlatMuon(FlatAdamW):
     ``adjust_lr_fn`` are those of ``torch.optim.Muon``, except that ``adjust_lr_fn`` defaults to
     ``"match_rms_adamw"``, since one learning rate drives both kinds; ``adamw_lr_ratio`` scales it for the AdamW part,
     whose other settings are ``betas`` and ``adamw_eps``.  ``matrix_filter(fqn, shape)`` decides which matrices are
-    orthogonalised (default :func:`is_hidden_matrix`).
+    orthogonalised (default: :func:`is_hidden_matrix`, and no weight of an ``nn.Embedding``).
 
     On one rank the matrices of one shape go through the kernels together, momentum, products and the new bf16 weights
     in one chain.  Across ranks a matrix lies in several shards: each rank updates its momentum, the unit's
@@ -129,9 +137,8 @@ class FlatMuon(FlatAdamW):
         self._ns = dict(steps=int(ns_steps), coefficients=tuple(float(c) for c in ns_coefficients))
         self._adjust = adjust_lr_fn
         self._adamw_lr_ratio = float(adamw_lr_ratio)
-        keep = matrix_filter if matrix_filter is not None else is_hidden_matrix
-        self._matrices = {id(u): [e for e in u.entries if len(e.shape) == 2 and e.numel and keep(e.fqns[0], tuple(e.shape))]
-                          for u in self.units}
+        keep = _is_hidden_entry if matrix_filter is None else lambda e: matrix_filter(e.fqns[0], tuple(e.shape))
+        self._matrices = {id(u): [e for e in u.entries if len(e.shape) == 2 and e.numel and keep(e)] for u in self.units}
 
     def _rest(self, u: Any) -> list[tuple[int, int]]:
         """The ranges of a unit's flat buffer that AdamW updates: what lies between the matrices.  A matrix ends
