@@ -126,7 +126,7 @@ class FlatMuon(FlatAdamW):
                  nesterov: bool = True, ns_coefficients: Sequence[float] = ops.NS_COEFFICIENTS, eps: float = ops.NS_EPS,
                  ns_steps: int = ops.NS_STEPS, adjust_lr_fn: Optional[str] = "match_rms_adamw",
                  betas: tuple[float, float] = (0.9, 0.95), adamw_eps: float = 1e-8, adamw_lr_ratio: float = 1.0,
-                 matrix_filter: Optional[Callable[[str, Sequence[int]], bool]] = None, **unused: Any) -> None:
+                 matrix_filter: Optional[Callable[[str, Sequence[int]], bool]] = None) -> None:
         if fsdp.tp_world > 1:
             raise ValueError("FlatMuon: matrices split over a tensor-parallel group are not supported")
         if not 0.0 <= momentum < 1.0:
