@@ -193,9 +193,30 @@ class _Linear(torch.autograd.Function):
         return dx, dw
 
 
+class _LinearInto(torch.autograd.Function):
+    """``F.linear`` whose weight gradient goes into an accumulator: for a weight that autograd does not track, such as
+    the view over several parameters that a fused projection multiplies by."""
+
+    @staticmethod
+    def forward(ctx, x, w, acc):
+        ctx.save_for_backward(x, w)
+        ctx.acc = acc
+        return F.linear(x, w.to(x.dtype))
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, w = ctx.saved_tensors
+        dy2, x2 = dy.reshape(-1, dy.shape[-1]), x.reshape(-1, x.shape[-1])
+        ctx.acc.add_(dy2.t().to(ctx.acc.dtype) @ x2.to(ctx.acc.dtype))
+        return dy @ w.to(dy.dtype), None, None
+
+
 def linear(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     """``x @ w.T`` (no bias) on the tcgen05 GEMM; eager ``F.linear`` on CPU."""
     if not _native(x):
+        acc = grad_acc(w)
+        if acc is not None and not w.requires_grad and torch.is_grad_enabled() and x.requires_grad:
+            return _LinearInto.apply(x, w, acc)
         return F.linear(x, w.to(x.dtype))
     if x.dtype != torch.bfloat16:
         x = x.to(torch.bfloat16)
