@@ -83,6 +83,7 @@ class FlatAdamW(torch.optim.Optimizer):
     def load_checkpoint_state_dict(self, sd: dict[str, Any], full: bool = False) -> None:
         state = sd.get("state", {})
         self.fsdp.load_optimizer_views(state)
+        self._check_second_moments()
         steps = [v["step"] for v in state.values() if isinstance(v, dict) and "step" in v]
         if steps:
             self._step_count = int(float(steps[0]))
@@ -91,6 +92,33 @@ class FlatAdamW(torch.optim.Optimizer):
             for k in ("lr", "betas", "eps", "weight_decay", "initial_lr"):
                 if k in groups[0]:
                     self.param_groups[0][k] = groups[0][k]
+
+    @torch.no_grad()
+    def _check_second_moments(self) -> None:
+        """Refuse first moments without second ones (a :class:`FlatMuon` checkpoint): AdamW would divide by their root.
+        The moments are then those of a fresh optimizer.
+
+        Every rank takes part and all refuse together.  First moments below 1e-15 prove nothing, their squares may have
+        underflowed."""
+        f = self.fsdp
+        names = [(u, e) for u in self.units for e in u.entries]
+        seen = torch.zeros(len(names), 2, device=f.device)
+        for i, (u, e) in enumerate(names):
+            lo, hi = u.local_range(f.rank)
+            a, b = max(e.offset, lo) - lo, min(e.offset + e.numel, hi) - lo
+            if a < b:
+                seen[i, 0], seen[i, 1] = u.exp_avg[a:b].abs().max(), u.exp_avg_sq[a:b].max()
+        for group, world in ((f.group, f.world), (f.tp_group, f.tp_world)):
+            if world > 1:
+                torch.distributed.all_reduce(seen, op=torch.distributed.ReduceOp.MAX, group=group)
+        first, second = seen.cpu().unbind(1)
+        bad = [e.fqns[0] for (_, e), x, y in zip(names, first.tolist(), second.tolist()) if x > 1e-15 and y == 0.0]
+        if bad:
+            for u in self.units:
+                u.exp_avg.zero_()
+                u.exp_avg_sq.zero_()
+            raise ValueError(f"FlatAdamW: the checkpoint holds no second moments of {bad[0]} and {len(bad) - 1} more "
+                             "parameters (written by FlatMuon?); resume it with Muon, or load the model alone")
 
 
 def is_hidden_matrix(fqn: str, shape: Sequence[int]) -> bool:
@@ -118,8 +146,8 @@ class FlatMuon(FlatAdamW):
     On one rank the matrices of one shape go through the kernels together, momentum, products and the new bf16 weights
     in one chain.  Across ranks a matrix lies in several shards: each rank updates its momentum, the unit's
     updates are gathered, and a rank orthogonalises the matrices that its shard holds a part of.  The momentum lives in
-    the first AdamW moment (``exp_avg`` in checkpoints); the second stays zero for matrices.  Matrices split over a
-    tensor-parallel group are not supported.
+    the first AdamW moment (``exp_avg`` in checkpoints); the second stays zero for matrices, also when an AdamW checkpoint
+    is loaded, and :class:`FlatAdamW` refuses such a checkpoint.  Matrices split over a tensor-parallel group are not supported.
     """
 
     def __init__(self, fsdp: NativeFSDP, lr: float = 1e-3, weight_decay: float = 0.1, momentum: float = 0.95,
@@ -231,11 +259,20 @@ class FlatMuon(FlatAdamW):
 
     def load_checkpoint_state_dict(self, sd: dict[str, Any], full: bool = False) -> None:
         super().load_checkpoint_state_dict(sd, full)
+        for u in self.units:  # an AdamW checkpoint's second moments of what Muon updates
+            lo, hi = u.local_range(self.fsdp.rank)
+            for e in self._matrices[id(u)]:
+                a, b = max(e.offset, lo) - lo, min(e.offset + e.numel, hi) - lo
+                if a < b:
+                    u.exp_avg_sq[a:b].zero_()
         groups = sd.get("param_groups") or []
         if groups:
             for k in ("momentum", "nesterov", "ns_eps"):
                 if k in groups[0]:
                     self.param_groups[0][k] = groups[0][k]
+
+    def _check_second_moments(self) -> None:
+        """Matrices have none here."""
 
     def _group_meta(self, fqns: list[str]) -> dict[str, Any]:
         g = self.param_groups[0]
