@@ -739,13 +739,15 @@ def adamw_step_(
 ) -> None:
     """Decoupled-weight-decay Adam on flat fp32 buffers, mirroring ``torch.optim.AdamW``
     (single-tensor path).  The gradient is multiplied by ``grad_scale`` and, when
-    ``norm_sq`` is given, by the clip coefficient ``min(1, max_norm / (sqrt(norm_sq)*grad_scale + 1e-6))``."""
+    ``norm_sq`` is given, by the clip coefficient ``min(1, max_norm / (sqrt(norm_sq)*grad_scale + 1e-6))``; a norm
+    that is not a number makes every weight so, as ``torch.nn.utils.clip_grad_norm_`` in front of the step does."""
     if not _native(p):
         with torch.no_grad():
             scale = grad_scale
             if norm_sq is not None:
                 total = float(norm_sq.sqrt()) * grad_scale
-                scale *= min(1.0, max_norm / (total + 1e-6))
+                clip = max_norm / (total + 1e-6)
+                scale *= 1.0 if clip > 1.0 else clip
             gg = g * scale
             p.mul_(1 - lr * weight_decay)
             m.lerp_(gg, 1 - beta1)

@@ -152,7 +152,7 @@ __global__ void adamw_kernel(AdamWArgs a) {
   if (a.norm_sq != nullptr) {
     const float total = sqrtf(*a.norm_sq) * a.grad_scale;
     const float coef = a.max_norm / (total + 1e-6f);
-    scale *= fminf(coef, 1.f);
+    scale *= (coef > 1.f) ? 1.f : coef;  // a NaN norm stays NaN
   }
   const float step_size = a.lr / a.bc1;
   const float decay = 1.f - a.lr * a.wd;

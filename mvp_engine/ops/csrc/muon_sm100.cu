@@ -603,7 +603,7 @@ __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// The gradient's factor: its scale times the global-norm clip coefficient (as in the AdamW kernel).
+// The gradient's factor: its scale times the global-norm clip coefficient (as in the AdamW kernel, NaN norms included).
 __device__ __forceinline__ float grad_factor(const StartParams& p) {
   float scale = p.grad_scale;
   if (p.norm_sq != nullptr) {
