@@ -592,7 +592,7 @@ struct StartParams {
   __half* lo;
   float sigma;
   double eps;
-  float momentum;
+  float momentum, one_minus;  // one_minus: 1 - momentum, taken in 64 bits
   int nesterov;
   float grad_scale;
   const float* norm_sq;
@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(kStartThreads) ns_norm_kernel(const __grid_con
     float u = gi;
     if constexpr (STEP) {
       gi *= scale;
-      mi = mi + (1.f - p.momentum) * (gi - mi);
+      mi = mi + p.one_minus * (gi - mi);
       u = p.nesterov ? gi + p.momentum * (mi - gi) : mi;
     }
     s += static_cast<double>(u) * u;
@@ -1108,6 +1108,7 @@ void muon_step_(const std::vector<torch::Tensor>& p, const std::vector<torch::Te
     auto partial = torch::empty({s.count, ctas}, p[0].options().dtype(at::kDouble));
     StartParams q = start_params(s, w, partial, eps);
     q.momentum = static_cast<float>(momentum);
+    q.one_minus = static_cast<float>(1.0 - momentum);
     q.nesterov = nesterov ? 1 : 0;
     q.grad_scale = static_cast<float>(grad_scale);
     q.norm_sq = norm_sq.has_value() ? norm_sq->data_ptr<float>() : nullptr;
