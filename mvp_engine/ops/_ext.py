@@ -16,7 +16,8 @@ import torch
 _EXT = None
 _ERR: Exception | None = None
 
-# Kernels launched per extension call (for launch accounting in benchmarks).
+# Kernels launched per extension call (for launch accounting in benchmarks): a number, or a function of the call's
+# positional arguments and result where they decide.
 KERNELS_PER_CALL = {
     "gemm": 1, "rmsnorm_fwd": 1, "rmsnorm_bwd": 2, "qk_norm_rope_fwd": 1, "qk_norm_rope_bwd": 1, "swiglu_fwd": 1,
     "swiglu_bwd": 1, "ce_fwd": 1, "ce_bwd_": 1, "adamw_step_": 1, "sumsq": 1, "embedding_fwd": 1,
@@ -26,8 +27,11 @@ KERNELS_PER_CALL = {
     "layernorm_fwd": 1, "layernorm_bwd": 3, "bias_gelu_fwd": 1, "bias_gelu_bwd": 2, "vision_rope_fwd": 1,
     "vision_rope_bwd": 1, "bias_residual_fwd": 1, "bias_grad": 2,
     "peer_gather_shards": 1, "publish_epoch": 1, "gemm_pair_gather": 1,
-    "quantize_fp8": 1, "gemm_fp8": 1, "linear_fp8_fwd": 3, "linear_fp8_bwd": 3,
-    "orthogonalize": 17, "muon_step_": 17,  # norm, first X and three products for each of five iterations
+    "quantize_fp8": 1, "gemm_fp8": 1,
+    "linear_fp8_fwd": lambda a, result: 2 if a[2] is not None else 3,  # a kept weight (w8) is not quantised
+    "linear_fp8_bwd": lambda a, result: 1 + (a[1] is not None) + (a[3] is not None),  # dw and dx, where asked for
+    "orthogonalize": lambda a, result: result,  # these two return it
+    "muon_step_": lambda a, result: result,
 }
 launch_count = 0
 counting = False
@@ -47,9 +51,10 @@ class _Counting:
 
         def wrapped(*a, **kw):
             global launch_count
+            result = fn(*a, **kw)
             if counting:
-                launch_count += k
-            return fn(*a, **kw)
+                launch_count += k(a, result) if callable(k) else k
+            return result
 
         self.__dict__[name] = wrapped  # found directly from now on
         return wrapped

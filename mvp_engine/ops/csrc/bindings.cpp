@@ -103,13 +103,13 @@ torch::Tensor bias_grad(const torch::Tensor& g, const c10::optional<torch::Tenso
 torch::Tensor vision_rope_bwd(const torch::Tensor& dq, const torch::Tensor& dk, const torch::Tensor& dv,
                               const torch::Tensor& cosv, const torch::Tensor& sinv, int64_t D);
 
-void orthogonalize(const torch::Tensor& x, torch::Tensor& out, int64_t steps, const std::vector<double>& coefficients,
-                   double eps, int64_t status_ptr);
-void muon_step_(const std::vector<torch::Tensor>& p, const std::vector<torch::Tensor>& g,
-                const std::vector<torch::Tensor>& mom, const std::vector<torch::Tensor>& p_bf16, double rate,
-                double decay, double momentum, bool nesterov, int64_t steps, const std::vector<double>& coefficients,
-                double eps, double grad_scale, const c10::optional<torch::Tensor>& norm_sq, double max_norm,
-                int64_t status_ptr);
+int64_t orthogonalize(const torch::Tensor& x, torch::Tensor& out, int64_t steps,
+                      const std::vector<double>& coefficients, double eps, int64_t status_ptr);
+int64_t muon_step_(const std::vector<torch::Tensor>& p, const std::vector<torch::Tensor>& g,
+                   const std::vector<torch::Tensor>& mom, const std::vector<torch::Tensor>& p_bf16, double rate,
+                   double decay, double momentum, bool nesterov, int64_t steps, const std::vector<double>& coefficients,
+                   double eps, double grad_scale, const c10::optional<torch::Tensor>& norm_sq, double max_norm,
+                   int64_t status_ptr);
 
 std::vector<torch::Tensor> quantize_fp8(const torch::Tensor& x, bool tile, bool rows, bool columns, bool e5m2);
 void gemm_fp8(const torch::Tensor& a, const torch::Tensor& sa, const torch::Tensor& b, const torch::Tensor& sb,

@@ -976,6 +976,9 @@ inline int64_t group_size(int64_t rows, int64_t cols, int64_t count) {
   return std::min<int64_t>(count, std::min<int64_t>(kMaxStack, fit));
 }
 
+// Norm, first X and three products an iteration.
+inline int64_t kernels_per_group(int64_t steps) { return 2 + 3 * steps; }
+
 inline StartParams start_params(const Shape& s, Workspace& w, torch::Tensor& partial, double eps) {
   StartParams q{};
   q.rows = s.rows;
@@ -1029,8 +1032,8 @@ void last_out(const Operand& ta, const Operand& tb, const Params& p, const Outs&
 }  // namespace muon
 }  // namespace mvp
 
-// O [count, m, n] of x [count, m, n] (contiguous fp32 / bf16 / fp16), in `out`'s type.
-void orthogonalize(const torch::Tensor& x, torch::Tensor& out, int64_t steps, const std::vector<double>& coefficients,
+// O [count, m, n] of x [count, m, n] (contiguous fp32 / bf16 / fp16), in `out`'s type.  Returns the kernels launched.
+int64_t orthogonalize(const torch::Tensor& x, torch::Tensor& out, int64_t steps, const std::vector<double>& coefficients,
                    double eps, int64_t status_ptr) {
   using namespace mvp::muon;
   TORCH_CHECK(x.is_cuda() && x.dim() == 3 && x.is_contiguous(), "orthogonalize: contiguous CUDA [count, m, n]");
@@ -1042,6 +1045,7 @@ void orthogonalize(const torch::Tensor& x, torch::Tensor& out, int64_t steps, co
   const int sms = mvp::num_sms(x.get_device());
   const int64_t size = x.size(1) * x.size(2);
   const int64_t group = group_size(x.size(1), x.size(2), x.size(0));
+  int64_t launched = 0;
   for (int64_t first = 0; first < x.size(0); first += group) {
     const Shape s(x.size(1), x.size(2), std::min<int64_t>(group, x.size(0) - first), out.scalar_type() == at::kFloat);
     Workspace w(s, x.device());
@@ -1066,17 +1070,20 @@ void orthogonalize(const torch::Tensor& x, torch::Tensor& out, int64_t steps, co
               else if (out.scalar_type() == at::kHalf) last_out<__half>(ta, tb, p, outs, s.tall, sms, stream);
               else TORCH_CHECK(false, "orthogonalize: fp32, bf16 or fp16 output");
             });
+    launched += kernels_per_group(steps);
   }
+  return launched;
 }
 
-// One step on same-shaped fp32 matrices p (master), g (gradient), mom (momentum); see ops.muon_step_.
-void muon_step_(const std::vector<torch::Tensor>& p, const std::vector<torch::Tensor>& g,
+// One step on same-shaped fp32 matrices p (master), g (gradient), mom (momentum); see ops.muon_step_.  Returns the kernels
+// launched.
+int64_t muon_step_(const std::vector<torch::Tensor>& p, const std::vector<torch::Tensor>& g,
                 const std::vector<torch::Tensor>& mom, const std::vector<torch::Tensor>& p_bf16, double rate,
                 double decay, double momentum, bool nesterov, int64_t steps, const std::vector<double>& coefficients,
                 double eps, double grad_scale, const c10::optional<torch::Tensor>& norm_sq, double max_norm,
                 int64_t status_ptr) {
   using namespace mvp::muon;
-  if (p.empty()) return;
+  if (p.empty()) return 0;
   const size_t count = p.size();
   TORCH_CHECK(g.size() == count && mom.size() == count && (p_bf16.empty() || p_bf16.size() == count),
               "muon_step_: one gradient, momentum (and bf16 copy) per weight");
@@ -1101,6 +1108,7 @@ void muon_step_(const std::vector<torch::Tensor>& p, const std::vector<torch::Te
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   const int sms = mvp::num_sms(dev.index());
   const int64_t group = group_size(sizes[0], sizes[1], static_cast<int64_t>(count));
+  int64_t launched = 0;
   for (int64_t first = 0; first < static_cast<int64_t>(count); first += group) {
     const Shape s(sizes[0], sizes[1], std::min<int64_t>(group, static_cast<int64_t>(count) - first), true);
     Workspace w(s, dev);
@@ -1130,5 +1138,7 @@ void muon_step_(const std::vector<torch::Tensor>& p, const std::vector<torch::Te
               if (s.tall) product<false, false, kStep>(ta, tb, l, outs, sms, stream);
               else product<false, true, kStep>(ta, tb, l, outs, sms, stream);
             });
+    launched += kernels_per_group(steps);
   }
+  return launched;
 }
