@@ -8,6 +8,22 @@ from mvp_engine import ops
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a GPU")]
 
 
+COEF = (3.4445, -4.7750, 2.0315)
+NS_TOL = 3e-3  # documented
+
+
+def ns64(u, steps, eps):
+    a, b, c = COEF
+    x = u.double()
+    x = x / max(float(x.norm()), eps)
+    tall = x.shape[0] > x.shape[1]
+    x = x.T if tall else x
+    for _ in range(steps):
+        s = x @ x.T
+        x = a * x + (b * s + c * s @ s) @ x
+    return x.T if tall else x
+
+
 def rand(shape, seed=0):
     return torch.randn(shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
 
@@ -39,3 +55,32 @@ def test_launches_are_counted_by_steps_and_groups():
     assert count(lambda: ops.linear_fp8(a, w)) == 3 and count(lambda: ops.linear_fp8(a, w, w8)) == 2
     assert count(lambda: ops.linear_fp8(a, w, w8).sum().backward()) == 4  # dx alone
     assert count(lambda: ops.linear_fp8(a, w.requires_grad_()).sum().backward()) == 6
+
+
+@pytest.mark.parametrize("shape", [(1, 9), (8, 8), (40, 72), (130, 64), (800, 1030)])
+@pytest.mark.parametrize("ratio", [3.0, 1.0, 1e-2, 1e-3, 1e-4, 1e-5, 1e-6, 1e-8, 1e-10, 1e-13])
+def test_norms_below_eps(shape, ratio):
+    """X is rounded to a step of 2^-24 in units in which |X|_F = 1 is at most sqrt(2) sqrt(m n): half a step in every
+    value of five X is sqrt(2) 2^-25 (a + .. + a^5) = 2.9e-5 of the result."""
+    x = rand(shape, 7)
+    x = x / x.norm() * 1e-4
+    eps = float(x.double().norm()) / ratio
+    want = ns64(x, 5, eps)
+    for dtype, half in ((torch.float32, 2.0**-24), (torch.bfloat16, 2.0**-8)):
+        got = ops.orthogonalize(x, eps=eps, out_dtype=dtype).double()
+        off = float((got - want).norm())
+        size = float(want.norm())
+        if ratio >= 1e-4:
+            assert off <= (NS_TOL + half) * size
+        else:
+            assert off <= 3e-5 + half * (size + 3e-5)
+
+
+@pytest.mark.parametrize("steps", [1, 5, 7, 12, 20, 50, 100, 200])
+@pytest.mark.parametrize("shape", [(192, 320), (1000, 333), (1024, 1536)])
+def test_many_steps(shape, steps):
+    """With these coefficients singular values keep moving within 0.7 to 1.2, and each step rounds them again."""
+    x = rand(shape, 3)
+    want = ns64(x, steps, 1e-7)
+    off = float((ops.orthogonalize(x, steps=steps, out_dtype=torch.float32).double() - want).norm())
+    assert off <= NS_TOL * max(1.0, steps / 5) ** 0.5 * float(want.norm())
