@@ -11,7 +11,7 @@ from __future__ import annotations
 
 from typing import Any, Literal, Optional
 
-from pydantic import BaseModel, ConfigDict, Field, field_validator
+from pydantic import BaseModel, ConfigDict, Field, field_validator, model_validator
 
 from mvp_engine.config.schema import BaseEngineConfig, BaseLoopConfig, BaseOptimConfig
 
@@ -124,6 +124,14 @@ class Qwen3Config(BaseEngineConfig):
     model: Qwen3ModelConfig = Field(default_factory=Qwen3ModelConfig)
     optim: Qwen3OptimConfig = Field(default_factory=Qwen3OptimConfig)
     loop: Qwen3LoopConfig = Field(default_factory=Qwen3LoopConfig)
+
+    @model_validator(mode="after")
+    def _precision_fits_mesh(self) -> "Qwen3Config":
+        mesh = self.parallel.mesh
+        if self.model.linear_precision == "fp8" and (mesh.tensor > 1 or mesh.context > 1):  # -1: known at the first forward
+            raise ValueError("`model.linear_precision: fp8` does not combine with `parallel.mesh.tensor` or "
+                             "`parallel.mesh.context` above 1.")
+        return self
 
     def resolve_batching_config(self, *, data_parallel_world_size: int) -> None:
         """Infer ``data.batch_size`` or ``optim.gradient_accumulation_steps`` (-1) from the global batch."""
