@@ -364,7 +364,8 @@ def run_ours(args) -> None:
         "higher_is_better": True,
         "scaling": "weak" if cp == 1 and "global_batch" not in wl else "strong",
         "vs_baseline": None,
-        "dtype": "bf16",
+        "dtype": ("bf16" if getattr(engine.config.model, "linear_precision", "bf16") == "bf16" else
+                  f"{engine.config.model.linear_precision} decoder projections, else bf16"),
         "data": (f"synthetic: 1-4 images per sample, sides multiples of 32 in [{lo},{hi}] px, N(0,1) pixels, "
                  f"interleaved with uniform-random text tokens, packed to {args.seq_len} tokens, loss on text "
                  f"positions; random-init {wl['model_name']} weights" if recipe == "qwen3_vl" else
@@ -376,7 +377,7 @@ def run_ours(args) -> None:
                    "micro_batch": 1, "grad_accum": ga, "workload": args.workload,
                    "activation_checkpoint_layers": ckpt_layers,
                    "l2": "no flush: weights, optimizer state and activations >> 126 MB L2",
-                   "optimizer": "AdamW (fp32 master, fused flat-shard kernel), clip 1.0, cosine"},
+                   "optimizer": f"{engine.config.optim.optimizer} (fp32 master, fused flat-shard kernel), clip 1.0, cosine"},
         "tokens_per_s_per_gpu": round(value / world, 1),
         "mfu": round(flops_per_step / (ms / 1e3) / (2250e12 * world), 4),
         "mfu_vs_measured_bf16_sustained": (round(flops_per_step / (ms / 1e3) / (peaks["bf16_tflops_sustained"] * 1e12
