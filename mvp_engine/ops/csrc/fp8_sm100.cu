@@ -12,8 +12,10 @@
 // spreads over the 4 x 32 lanes of tensor memory, so the product loads scales with plain 512-byte copies.
 //
 // Quantisation reads a matrix once and writes the codes of its rows, of its columns (the transposed matrix, blocks
-// along the former rows), or both.  It is bound by memory: 2 bytes read and 1 or 2 written per bf16 value.  Measured, both
-// orientations: 8192 x 4096 in 32 us (4.2 TB/s), 8192 x 12288 in 67 us (6.0 TB/s).
+// along the former rows), or both.  Its floor is memory: 2 bytes read and 1 or 2 written per bf16 value.  Measured, row blocks,
+// both orientations: 8192 x 4096 in 29 us (4.6 TB/s; fp32 values 42 us, 4.8), 8192 x 12288 in 74 us (5.4 TB/s; fp32 114 us, 5.3);
+// 128 x 128 tiles 27 and 68 us; e5m2 as e4m3.  Below some tens of millions of values the few waves of CTAs, whose load, reduction
+// and store follow one another, keep it off the copy rate (6.45).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
@@ -374,8 +376,10 @@ void quantize(const QuantParams& p, bool e5m2, bool tile, int ctas, bool early, 
 // tile two before has been read out), so at least 10 k-blocks do, more than the ring's stages: the full
 // stage that the new group waits for was emptied after the old group's MMAs.
 //
-// Bound by the tensor core, and for long runs by the power limit: 8192 x 4096 -> 24576 in 562 us (2.93 PFLOP/s, 0.87 of twice
-// the bf16 rate measured on the same GPU), 8192 x 12288 -> 4096 in 270 us (3.05 PFLOP/s).
+// Bound by the tensor core, and for long runs by the power limit: 8192 x 4096 -> 24576 in 560 to 585 us in short runs (2.8 to
+// 2.9 PFLOP/s, 0.87 of twice the bf16 rate measured on the same GPU) and 660 to 690 us in long ones (2.4 to 2.5),
+// 8192 x 12288 -> 4096 in 270 to 280 and 325 us.  Adding into an fp32 C costs 9 to 25 % more: its rows are read behind the
+// accumulator, and the ring is one stage shorter.
 namespace fp8gemm {
 
 using namespace gemm2;
@@ -758,8 +762,12 @@ inline void encode(CUtensorMap* map, CUtensorMapDataType type, const void* base,
 
 // Tile width with the shortest schedule: waves x (cycles of a tile: its k-blocks, plus what it costs besides), and the last
 // tile's read-out.  A k-block of 128 takes 2 TN cycles at the tensor core's rate and a little more where A's share of the
-// shared-memory traffic grows.  Measured: 8192 x 4096 -> 24576 in 562 us with 192 columns, 600 with 256 (the hand-over
-// of the shared columns); 8192 x 4096 -> 4096 in 99 us with 256 (7 waves) and 153 with 128 (14 waves).
+// shared-memory traffic grows.  Measured with each width in turn (us at 256 / 192 / 128 columns, bf16 result):
+//   256 x 4096 -> 4096   15.9 / 13.1 / 11.6     8192 x 4096 -> 4096    106 / 109 / 128
+//   777 x 2560 -> 9728   25.4 / 20.5 / 25.3     8192 x 4096 -> 24576   694 / 665 / 836  (256: hand-over of the shared columns)
+//   4096 x 4096 -> 4096  66.7 / 61.9 / 70.5     8192 x 12288 -> 4096   328 / 349 / 402
+// Over 14 such shapes the choice is within 1 % of the best, and within 8 % where C is added to in fp32 (8192 x 4096 -> 12288:
+// 388 at 256 columns, 408 at the chosen 192), whose longer read-out it does not weigh.
 inline int choose_tile(int64_t M, int64_t N, int num_kb, int sms) {
   const int64_t clusters = std::max(1, sms / 2);
   struct Width {

@@ -32,9 +32,9 @@
 // tile and its mirror, which makes an iteration s^2 l + s^3 + 2 s^2 l operations instead of 4 s^2 l + 2 s^3.
 // One launch per product handles a whole stack of same-shaped matrices.  The kernel is the pair-of-SMs GEMM
 // (256 x 256 or 256 x 128 tile per cluster, see gemm2sm_sm100.cu for the roles) over 3-D tensor maps.
-// Measured, five iterations: 4 x 4096 x 4096 in 4.3 to 4.7 ms (1.2 to 1.3 PFLOP/s; the bf16 GEMM settles at 1.4 under the
-// power limit), 12 x 1024 x 4096 in 1.1 ms, bound by what X's update moves through L2 (4 bytes read and 4 written per value
-// beside the operands), 1 x 256 x 512 in 105 us, bound by 17 dependent launches.
+// Measured, five iterations: 4 x 4096 x 4096 in 4.5 ms in short runs and 5.1 ms in long ones under the power limit (1.2 and 1.1
+// PFLOP/s; the bf16 GEMM settles at 1.4), 12 x 1024 x 4096 in 1.2 ms, bound by what X's update moves through L2 (4 bytes read
+// and 4 written per value beside the operands), 1 x 256 x 512 in 104 us, bound by 17 dependent launches.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -807,8 +807,11 @@ inline int64_t tiles_of(bool sym, int M, int N, int tn) {
 // Tile width with the shorter schedule.  A tile's MMAs take 512 cycles per k-block at TN = 256 and about 350 at 128 (A's share
 // of the shared-memory traffic grows); its read-out, which overlaps the next tile's MMAs, about 5500 cycles (A),
 // 9500 (B) and 12500 (X) at 256 and half of that at 128 (both from time stamps of single tiles).  Beyond two waves of the
-// narrow tiles memory sets the pace and the wide ones win (12 x 1024 x 4096: 1.16 ms wide, 1.23 ms narrow; a Muon step on
-// 3 x 1001 x 777: 267 us wide, 202 us narrow).
+// narrow tiles memory sets the pace and the wide ones win.  Measured, whole iterations (us, wide / narrow / chosen per product):
+//   1 x 256 x 512    139 / 103 / 103     2 x 1024 x 4096    352 / 303 / 289      2 x 2048 x 2048   435 / 497 / 436
+//   1 x 1024 x 1024  225 / 159 / 159     4 x 1024 x 4096    480 / 549 / 473      1 x 4096 x 4096  1352 / 1720 / 1350
+//   3 x 1001 x 777   249 / 201 / 201     12 x 1024 x 4096  1223 / 1551 / 1220    12 x 512 x 2048   324 / 280 / 273
+// The worst of 16 such stacks is 6 x 1001 x 777: 283 chosen, 268 with narrow tiles throughout.
 inline int choose_tile(bool sym, bool reads, int M, int N, int K, int count, int sms) {
   const int64_t clusters = std::max(1, sms / 2), kb = (K + BK - 1) / BK;
   int64_t cost[2], waves = 0;
@@ -877,7 +880,7 @@ struct Shape {
   float sigma, tau;
   // `fine`: the result keeps more than 16 bits.  The error falls with the long side (simulated against 64 bits: 6e-4 at 200 x 200,
   // 4.9e-4 at 400 x 500, 4.1e-4 at 128 x 1000; with the low part 3.8e-4, 3.2e-4, 3.3e-4), while the extra passes cost least
-  // where a product is mostly start and end.
+  // where a product is mostly start and end (measured: 4 x 768 x 512 in 178 us with them, 144 without; 1 x 256 x 512 125 and 104).
   Shape(int64_t m, int64_t n, int64_t L, bool fine)
       : rows(static_cast<int>(m)), cols(static_cast<int>(n)), count(static_cast<int>(L)) {
     tall = m > n;
