@@ -22,9 +22,9 @@
 // only what is off them is rounded to fp16: with A = D + A~, A A = A~ A~ + (D_i + D_j) A~ + D^2 element by element, and
 // B's diagonal joins the linear term, (a + B_ii) (hi + lo).  That halves the error of well conditioned matrices
 // (simulated against 64 bits at 512 x 2048: 1.7e-3 -> 0.5e-3) and bounds it for tiny ones.
-// For small matrices, whose errors average less, a result that keeps more than 16 bits (the fp32 step or output) takes X's low
-// part into its products as well: (hi + lo)(hi + lo)^T without lo lo^T, and B (hi + lo), as two more passes and one more
-// over the reduction (Shape::split).
+// A result that keeps more than 16 bits (the fp32 step or output) shows more of that error, small matrices most, whose roundings
+// average less.  There X's low part enters the products as well, (hi + lo)(hi + lo)^T without lo lo^T and B (hi + lo), as more
+// passes over the reduction (Shape::split), and A and B off their diagonals are kept as hi + lo too (Shape::split_s).
 // Entries then stay below 1.9 sigma and 3.9 tau (the caller checks the coefficients for it), within 65504, and
 // what underflows is 2^-24 of an average entry.
 //
@@ -92,7 +92,7 @@ struct Params {
   const __half* C_hi;   // element-wise term, row stride ld, matrix stride ld * M
   const __half* C_lo;
   __half* D_hi;
-  __half* D_lo;
+  __half* D_lo;         // null: A and B have no low parts
   int ld;               // of C and D (a multiple of 8, at least N)
   float* diag;          // [count, ld_s] diagonal of D (kGram, kPoly: written, and zeroed in D) or of B (others: added
   int ld_s;             // to beta, times diag_scale, for row m where X is short by rows, else for column n)
@@ -165,12 +165,14 @@ __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-template <bool A_MN, bool B_MN, int EPI, typename OUT, int TN>
+// LOW: C and D have low parts (always so for X; for A and B where Shape::split_s is set).
+template <bool A_MN, bool B_MN, int EPI, typename OUT, int TN, bool LOW>
 __global__ void __launch_bounds__(THREADS, 1)
     ns_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                       const __grid_constant__ CUtensorMap tmA_low, const __grid_constant__ CUtensorMap tmB_low,
                       const Params p, const __grid_constant__ Outs outs) {
   constexpr bool SYM = EPI == kGram || EPI == kPoly;
+  static_assert(SYM || LOW, "X has a low part");
   constexpr int B_BYTES = kStageBytes<TN> - A_BYTES;
   constexpr int CHUNKS = TN / 2 / CHUNK;  // per epilogue warp and tile
   extern __shared__ uint8_t smem_raw[];
@@ -348,7 +350,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int64_t at = ok ? mat + static_cast<int64_t>(m) * p.ld + n : 0;
             const uint32_t d = dst + piece16(r, lane & 3);
             cp_async_16(d, p.C_hi + at, ok ? 16 : 0);
-            if constexpr (!SYM) cp_async_16(d + HALF_BUF, p.C_lo + at, ok ? 16 : 0);
+            if constexpr (LOW) cp_async_16(d + HALF_BUF, p.C_lo + at, ok ? 16 : 0);
           }
         }
         cp_async_commit();
@@ -403,13 +405,13 @@ __global__ void __launch_bounds__(THREADS, 1)
               const uint8_t* at = buf + piece16(lane, v);
               const uint4 hi = *reinterpret_cast<const uint4*>(at);
               uint4 lo = make_uint4(0u, 0u, 0u, 0u);
-              if constexpr (!SYM) lo = *reinterpret_cast<const uint4*>(at + HALF_BUF);
+              if constexpr (LOW) lo = *reinterpret_cast<const uint4*>(at + HALF_BUF);
               const uint32_t* hw = &hi.x;
               const uint32_t* lw = &lo.x;
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
                 float2 e = h2f(hw[q]);
-                if constexpr (!SYM) {
+                if constexpr (LOW) {
                   const float2 f = h2f(lw[q]);
                   e.x += f.x;
                   e.y += f.y;
@@ -458,7 +460,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               }
               uint8_t* at = buf + piece16(lane, v);
               *reinterpret_cast<uint4*>(at) = make_uint4(h[0], h[1], h[2], h[3]);
-              if constexpr (!SYM) *reinterpret_cast<uint4*>(at + HALF_BUF) = make_uint4(l[0], l[1], l[2], l[3]);
+              if constexpr (LOW) *reinterpret_cast<uint4*>(at + HALF_BUF) = make_uint4(l[0], l[1], l[2], l[3]);
             }
             __syncwarp();
 #pragma unroll
@@ -468,11 +470,13 @@ __global__ void __launch_bounds__(THREADS, 1)
               if (m_warp + r < p.M && col < p.ld) {
                 const int64_t d = mat + static_cast<int64_t>(m_warp + r) * p.ld + col;
                 *reinterpret_cast<uint4*>(p.D_hi + d) = *reinterpret_cast<const uint4*>(at);
-                if constexpr (!SYM) *reinterpret_cast<uint4*>(p.D_lo + d) = *reinterpret_cast<const uint4*>(at + HALF_BUF);
+                if constexpr (LOW)
+                  *reinterpret_cast<uint4*>(p.D_lo + d) = *reinterpret_cast<const uint4*>(at + HALF_BUF);
               }
             }
             if constexpr (SYM) {
               if (tn * TN + TN <= tm * TM && row_ok) {  // mirror: a warp's 32 rows are 64 contiguous bytes of each mirrored row
+                // (low parts are kept of matrices that are one block only, and no block is below the diagonal there)
                 __half* d = p.D_hi + mat + static_cast<int64_t>(n) * p.ld + m;
 #pragma unroll
                 for (int j = 0; j < CHUNK; ++j)
@@ -782,7 +786,7 @@ __global__ void __launch_bounds__(kStartThreads) ns_first_kernel(const __grid_co
 struct Operand {
   const __half* base;
   int cols, rows, ld;
-  const __half* low = nullptr;  // X's low part, where products read it
+  const __half* low = nullptr;  // its low part, where products read it
 };
 
 // Its tensor map; mn_major: boxes of 64 columns x BK rows, else of 64 columns (the reduction) x box_rows rows.
@@ -824,7 +828,7 @@ inline int choose_tile(bool sym, bool reads, int M, int N, int K, int count, int
   return waves <= 2 && cost[1] < cost[0] ? 128 : 256;
 }
 
-template <bool A_MN, bool B_MN, int EPI, typename OUT, int TN>
+template <bool A_MN, bool B_MN, int EPI, typename OUT, int TN, bool LOW>
 void launch(const Operand& a, const Operand& b, Params p, const Outs& outs, int sms, cudaStream_t stream) {
   CUtensorMap ta, tb;
   make_map(&ta, a, false, p.count, A_MN, HALF);
@@ -832,18 +836,18 @@ void launch(const Operand& a, const Operand& b, Params p, const Outs& outs, int 
   CUtensorMap ta_low = ta, tb_low = tb;
   p.passes = 1;
   p.low_a = p.low_b = 0;
-  if (a.low != nullptr && b.low != nullptr) {  // X X^T: hi hi, hi lo, lo hi
+  if (a.low != nullptr && b.low != nullptr) {  // X X^T, A A, B X: hi hi, hi lo, lo hi
     p.passes = 3;
     p.low_a = 0b100;
     p.low_b = 0b010;
-  } else if (a.low != nullptr || b.low != nullptr) {  // B X: hi, lo
+  } else if (a.low != nullptr || b.low != nullptr) {  // B X with one of them split: hi, lo
     p.passes = 2;
     p.low_a = p.low_b = 0b10;
   }
   if (a.low != nullptr) make_map(&ta_low, a, true, p.count, A_MN, HALF);
   if (b.low != nullptr) make_map(&tb_low, b, true, p.count, B_MN, TN / 2);
   p.tiles = static_cast<int>(tiles_of(EPI == kGram || EPI == kPoly, p.M, p.N, TN));
-  auto kern = ns_product_kernel<A_MN, B_MN, EPI, OUT, TN>;
+  auto kern = ns_product_kernel<A_MN, B_MN, EPI, OUT, TN, LOW>;
   static std::atomic<uint64_t> configured{0};
   allow_smem(kern, kSmemBytes<TN>, configured);
   cudaLaunchConfig_t cfg = {};
@@ -865,42 +869,57 @@ void launch(const Operand& a, const Operand& b, Params p, const Outs& outs, int 
 
 template <bool A_MN, bool B_MN, int EPI, typename OUT = float>
 void product(const Operand& a, const Operand& b, const Params& p, const Outs& outs, int sms, cudaStream_t stream) {
+  constexpr bool SYM = EPI == kGram || EPI == kPoly;
   const int passes = a.low != nullptr && b.low != nullptr ? 3 : a.low != nullptr || b.low != nullptr ? 2 : 1;
-  if (choose_tile(EPI == kGram || EPI == kPoly, EPI != kGram, p.M, p.N, passes * p.K, p.count, sms) == 256)
-    launch<A_MN, B_MN, EPI, OUT, 256>(a, b, p, outs, sms, stream);
-  else
-    launch<A_MN, B_MN, EPI, OUT, 128>(a, b, p, outs, sms, stream);
+  const bool wide = choose_tile(SYM, EPI != kGram, p.M, p.N, passes * p.K, p.count, sms) == 256;
+  if (!SYM || p.D_lo != nullptr) {
+    if (wide) launch<A_MN, B_MN, EPI, OUT, 256, true>(a, b, p, outs, sms, stream);
+    else launch<A_MN, B_MN, EPI, OUT, 128, true>(a, b, p, outs, sms, stream);
+  } else if constexpr (SYM) {
+    if (wide) launch<A_MN, B_MN, EPI, OUT, 256, false>(a, b, p, outs, sms, stream);
+    else launch<A_MN, B_MN, EPI, OUT, 128, false>(a, b, p, outs, sms, stream);
+  }
 }
 
 struct Shape {
   int rows, cols, count;
   int short_side, ldx, lds;
   bool tall;
-  bool split;  // X's low part takes part in the products
+  bool split;    // X's low part takes part in the products
+  bool split_s;  // A's and B's low parts are kept and take part in the products
   float sigma, tau;
-  // `fine`: the result keeps more than 16 bits.  The error falls with the long side (simulated against 64 bits: 6e-4 at 200 x 200,
-  // 4.9e-4 at 400 x 500, 4.1e-4 at 128 x 1000; with the low part 3.8e-4, 3.2e-4, 3.3e-4), while the extra passes cost least
-  // where a product is mostly start and end (measured: 4 x 768 x 512 in 178 us with them, 144 without; 1 x 256 x 512 125 and 104).
+  // `fine`: the result keeps more than 16 bits.  The error of the update falls with both sides, while the extra passes cost
+  // least where a product is mostly start and end, and those of A and B next to nothing where they are one k-block.  Measured on
+  // stacks of three, error against 64 bits and time, without low parts / X's / A's and B's / both (* what is taken):
+  //   8 x 16      1.1e-3  8.1e-4  1.0e-3  8e-7*     69   72   73   77 us
+  //   64 x 64     7.5e-4  4.5e-4  5.7e-4  1e-6*     82   86   90   93 us
+  //   64 x 512    4.9e-4  4.1e-4  2.7e-4* 4e-6      94  112  101  119 us
+  //   8 x 4096    5.0e-4  5.2e-4  2.1e-4* 7e-5     151  284  158  291 us
+  //   128 x 512   4.7e-4  3.5e-4* 3.1e-4  4e-6     104  121  119  137 us
+  //   256 x 256   6.1e-4  3.8e-4* 4.7e-4  2e-6     105  117  125  138 us
+  //   128 x 4096  3.8e-4* 3.4e-4  1.8e-4  4e-5     175  306  190  323 us
+  // Larger matrices end at 2e-4 to 5e-4 without any of it.
   Shape(int64_t m, int64_t n, int64_t L, bool fine)
       : rows(static_cast<int>(m)), cols(static_cast<int>(n)), count(static_cast<int>(L)) {
     tall = m > n;
-    split = fine && std::max(m, n) <= 768;
     short_side = tall ? cols : rows;
+    split_s = fine && short_side <= BK;
+    split = fine && std::max(m, n) <= (split_s ? 256 : 768);
     ldx = (cols + 7) / 8 * 8;
     lds = (short_side + 7) / 8 * 8;
     sigma = std::ldexp(1.f, static_cast<int>(std::min(15.0, std::round(0.5 * std::log2(static_cast<double>(m) * n)))));
     tau = std::ldexp(1.f, static_cast<int>(std::min(14.0, std::round(std::log2(static_cast<double>(short_side))))));
   }
   // fp16 elements of the workspace: X hi twice (a product reads one while its epilogue writes the other), X lo (twice too
-  // where products read it), A, B
+  // where products read it), A and B (and their low parts)
   int64_t x_elems() const { return static_cast<int64_t>(count) * rows * ldx; }
   int64_t s_elems() const { return static_cast<int64_t>(count) * short_side * lds; }
-  int64_t elems() const { return (split ? 4 : 3) * x_elems() + 2 * s_elems(); }
+  int64_t elems() const { return (split ? 4 : 3) * x_elems() + (split_s ? 4 : 2) * s_elems(); }
 };
 
 struct Workspace {
   torch::Tensor buf;
-  __half *hi[2], *lo[2], *A, *B;
+  __half *hi[2], *lo[2], *A, *B, *A_lo, *B_lo;
   float *diag_a, *diag_b;
   Workspace(const Shape& s, const torch::Device& dev) {
     const int64_t diag_elems = 4 * static_cast<int64_t>(s.count) * s.lds;  // two vectors of fp32
@@ -911,7 +930,9 @@ struct Workspace {
     lo[1] = s.split ? lo[0] + s.x_elems() : lo[0];
     A = lo[1] + s.x_elems();
     B = A + s.s_elems();
-    diag_a = reinterpret_cast<float*>(B + s.s_elems());
+    A_lo = s.split_s ? B + s.s_elems() : nullptr;
+    B_lo = s.split_s ? A_lo + s.s_elems() : nullptr;
+    diag_a = reinterpret_cast<float*>((s.split_s ? B_lo : B) + s.s_elems());
     diag_b = diag_a + static_cast<int64_t>(s.count) * s.lds;
   }
 };
@@ -921,7 +942,7 @@ template <typename Last>
 void iterate(const Shape& s, Workspace& w, int steps, double a, double b, double c, int* status, int sms,
              cudaStream_t stream, Last last) {
   const Outs none{};
-  const Operand A{w.A, s.short_side, s.short_side, s.lds}, B{w.B, s.short_side, s.short_side, s.lds};
+  const Operand A{w.A, s.short_side, s.short_side, s.lds, w.A_lo}, B{w.B, s.short_side, s.short_side, s.lds, w.B_lo};
   for (int it = 0; it < steps; ++it) {
     const int cur = it & 1;
     const Operand X{w.hi[cur], s.cols, s.rows, s.ldx, s.split ? w.lo[cur] : nullptr};
@@ -937,6 +958,7 @@ void iterate(const Shape& s, Workspace& w, int steps, double a, double b, double
     p.alpha = s.tau / s.sigma / s.sigma;
     p.beta = 0.f;
     p.D_hi = w.A;
+    p.D_lo = w.A_lo;
     p.diag = w.diag_a;
     if (s.tall) product<true, true, kGram>(X, X, p, none, sms, stream);
     else product<false, false, kGram>(X, X, p, none, sms, stream);
@@ -945,7 +967,9 @@ void iterate(const Shape& s, Workspace& w, int steps, double a, double b, double
     p.alpha = static_cast<float>(c / s.tau);
     p.beta = static_cast<float>(b);
     p.C_hi = w.A;
+    p.C_lo = w.A_lo;
     p.D_hi = w.B;
+    p.D_lo = w.B_lo;
     p.gamma = static_cast<float>(c);
     p.diag_a = w.diag_a;
     p.diag = w.diag_b;

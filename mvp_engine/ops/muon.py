@@ -75,10 +75,11 @@ def orthogonalize(x: torch.Tensor, *, steps: int = NS_STEPS, coefficients: Seque
 
     ``X = x / max(|x|_F, eps)``, then ``steps`` times ``X <- a X + (b A + c A A) X`` with ``A = X X^T`` over the
     shorter side.  ``x`` is fp32, bf16 or fp16; the result has ``out_dtype`` (one of the three).  On CUDA it is within
-    0.3 % (Frobenius) of 64-bit arithmetic plus its own rounding in up to five steps, and ``sqrt(steps / 5)`` times that in
-    more, where ``|x|_F`` is at least ``1e-4 eps``; smaller matrices, whose first X is that far below 1, keep fewer bits of
-    fp16: what they lose is below 3e-5 (Frobenius, five steps of the default coefficients).  A matrix with a value that is
-    not finite comes back as NaN, a zero matrix as zeros.  No gradient is defined.
+    0.3 % (Frobenius) of 64-bit arithmetic plus its own rounding in up to five steps (an fp32 result of sides up to 256, the
+    shorter up to 64: 0.03 %), and ``sqrt(steps / 5)`` times that in more, where ``|x|_F`` is at least ``1e-4 eps``.  Smaller
+    matrices, whose first X is that far below 1, keep fewer bits of fp16: what they lose is below 3e-5 (Frobenius, five steps
+    of the default coefficients).  A matrix with a value that is not finite comes back as NaN, a zero matrix as zeros.  No
+    gradient is defined.
     """
     if x.dim() < 2:
         raise ValueError(f"orthogonalize: matrices are needed, got shape {tuple(x.shape)}")

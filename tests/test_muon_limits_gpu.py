@@ -1,4 +1,10 @@
-"""The edges of what is documented for the Newton-Schulz kernels on the GPU."""
+"""The edges of what is documented for the Newton-Schulz kernels on the GPU.
+
+FINE_TOL, of fp32 results with sides up to 256, the shorter up to 64.  X, A and B are kept to 22 bits there, and no product
+drops more than lo lo.  What is left: sums of l / 16 partial sums in 32 bits (a step of 2^-23 each, in one direction if the
+hardware cuts off), three passes of 16 x 2^-23 of A in five iterations at l = 256, 3e-5; and an error of 2^-21 of B X in the strong directions,
+passed on to the weak ones at most 3.44^4 = 140 times, 7e-5 of the strongest singular value.  Three times the sum.
+"""
 
 import pytest
 import torch
@@ -10,6 +16,7 @@ pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(),
 
 COEF = (3.4445, -4.7750, 2.0315)
 NS_TOL = 3e-3  # documented
+FINE_TOL = 3e-4
 
 
 def ns64(u, steps, eps):
@@ -84,3 +91,47 @@ def test_many_steps(shape, steps):
     want = ns64(x, steps, 1e-7)
     off = float((ops.orthogonalize(x, steps=steps, out_dtype=torch.float32).double() - want).norm())
     assert off <= NS_TOL * max(1.0, steps / 5) ** 0.5 * float(want.norm())
+
+
+SMALL = [(1, 1), (1, 9), (9, 1), (8, 8), (8, 16), (16, 8), (33, 70), (64, 64), (63, 65), (64, 256), (256, 64), (8, 250),
+         (200, 3)]
+
+
+@pytest.mark.parametrize("shape", SMALL)
+@pytest.mark.parametrize("power", [0.0, -1.0, -4.0])
+def test_small_fp32_results_keep_more(shape, power):
+    x = rand((3, *shape), 5)
+    if power:  # singular values that decay as k ** power
+        u, d, v = torch.linalg.svd(x.double(), full_matrices=False)
+        x = ((u * torch.arange(1, d.shape[-1] + 1, device="cuda").double() ** power) @ v).float()
+    got = ops.orthogonalize(x, out_dtype=torch.float32).double()
+    for i in range(3):
+        want = ns64(x[i], 5, 1e-7)
+        assert float((got[i] - want).norm()) <= FINE_TOL * float(want.norm())
+
+
+@pytest.mark.parametrize("shape", SMALL)
+def test_small_steps_keep_the_weights_bits(shape):
+    n = 3
+    p, g, m = ([rand(shape, 50 + 10 * k + i) * s for i in range(n)] for k, s in enumerate((0.02, 1e-3, 1e-3)))
+    want = []
+    for pi, gi, mi in zip(p, g, m):
+        pi, gi, mi = pi.double(), gi.double(), mi.double()
+        mi = mi + 0.05 * (gi - mi)
+        move = 2e-4 * 0.2 * max(shape) ** 0.5 * ns64(gi + 0.95 * (mi - gi), 5, 1e-7)
+        want.append((pi * (1 - 2e-4 * 0.1) - move, move))
+    ops.muon_step_(p, g, m, lr=2e-4, weight_decay=0.1, adjust_lr="match_rms_adamw")
+    for got, (w, move) in zip(p, want):
+        assert float((got.double() - w).norm()) <= FINE_TOL * float(move.norm()) + 2.0**-23 * float(w.norm())
+
+
+@pytest.mark.parametrize("shape", [(257, 257), (256, 769), (769, 256), (16, 3000), (3000, 16), (64, 4096), (300, 700), (65, 65),
+                                   (64, 257), (257, 64), (65, 256), (8, 257), (65, 769)])
+def test_fp32_results_beyond(shape):
+    """A side beyond one of the two limits: the documented bound, and one matrix as in a stack."""
+    x = rand((2, *shape), 9)
+    got = ops.orthogonalize(x, out_dtype=torch.float32)
+    for i in range(2):
+        want = ns64(x[i], 5, 1e-7)
+        assert float((got[i].double() - want).norm()) <= NS_TOL * float(want.norm())
+        assert torch.equal(ops.orthogonalize(x[i], out_dtype=torch.float32), got[i])
