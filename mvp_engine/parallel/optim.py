@@ -101,7 +101,7 @@ class FlatAdamW(torch.optim.Optimizer):
         Every rank takes part and all refuse together.  First moments below 1e-15 prove nothing, their squares may have
         underflowed."""
         f = self.fsdp
-        names = [(u, e) for u in self.units for e in u.entries]
+        names = [(u, e) for u in self.units for e in u.entries if self._has_second_moment(u, e)]
         seen = torch.zeros(len(names), 2, device=f.device)
         for i, (u, e) in enumerate(names):
             lo, hi = u.local_range(f.rank)
@@ -117,8 +117,12 @@ class FlatAdamW(torch.optim.Optimizer):
             for u in self.units:
                 u.exp_avg.zero_()
                 u.exp_avg_sq.zero_()
-            raise ValueError(f"FlatAdamW: the checkpoint holds no second moments of {bad[0]} and {len(bad) - 1} more "
-                             "parameters (written by FlatMuon?); resume it with Muon, or load the model alone")
+            raise ValueError(f"{type(self).__name__}: the checkpoint holds no second moments of {bad[0]} and {len(bad) - 1} more "
+                             "parameters; Muon wrote it (resume with Muon and the same matrix_filter, or load the model alone)")
+
+    def _has_second_moment(self, u: Any, e: Any) -> bool:
+        """Whether AdamW updates this entry."""
+        return True
 
 
 def is_hidden_matrix(fqn: str, shape: Sequence[int]) -> bool:
@@ -271,8 +275,8 @@ class FlatMuon(FlatAdamW):
                 if k in groups[0]:
                     self.param_groups[0][k] = groups[0][k]
 
-    def _check_second_moments(self) -> None:
-        """Matrices have none here."""
+    def _has_second_moment(self, u: Any, e: Any) -> bool:
+        return not any(e is m for m in self._matrices[id(u)])
 
     def _group_meta(self, fqns: list[str]) -> dict[str, Any]:
         g = self.param_groups[0]

@@ -71,6 +71,17 @@ def test_other_pairs_load(world, wrote, reads):
     assert got == [""] * world
 
 
+def test_muon_refuses_what_another_filter_orthogonalised():
+    a, oa = build("FlatMuon")
+    steps(a, oa, 2)
+    osd = oa.checkpoint_state_dict(full=True)
+    ob = optim.FlatMuon(build("FlatMuon")[0], lr=1e-3, matrix_filter=lambda fqn, shape: "mlp" in fqn)
+    with pytest.raises(ValueError, match="matrix_filter"):
+        ob.load_checkpoint_state_dict(osd, full=True)
+    oc = optim.FlatMuon(build("FlatMuon")[0], lr=1e-3, matrix_filter=lambda fqn, shape: "norm" not in fqn)
+    oc.load_checkpoint_state_dict(osd, full=True)  # more matrices than before need no second moments
+
+
 def test_a_fresh_or_untouched_state_loads():
     """Zero moments on both sides, and first moments whose squares underflow."""
     a, oa = build("FlatAdamW")
